@@ -150,6 +150,35 @@ int64_t ppml_b200_q8_0r_bytes(int64_t numel);
 /* repack_q8_0_host on the device: 34-byte Q8_0 blocks (device, 2-byte aligned) -> planar Q8_0R (device, 4-byte aligned). */
 int ppml_b200_repack_q8_0(const void* blocks34_dev, int64_t nblocks, void* q8_0r_dev, void* stream);
 
+/* ---- Linear in 8-bit integers, one scale per token and one per output channel -------------------------------------
+ * No counterpart in the reference, whose only integer product scales every block of 32 (mul_mat_q8_cuda above).  With one
+ * scale per row on either side the whole sum over K stays in int32 on the tensor cores.
+ *   scale[t] = max_k |x[t][k]| / 127,  q[t][k] = clamp(round-half-even(x[t][k] / scale[t]), -127, 127)   (both quotients fp32)
+ *   C[m][n]  = act(a_scale[m] * b_scale[n] * sum_k A[m][k] * B[n][k] + bias[n]) * gate[m][n]
+ * A row of zeros has scale 0; a row that holds an infinity or a NaN has scale NaN and integers 0, so that its results are
+ * NaN and no other row's are touched.  The sum is exact for every K up to PPML_B200_I8_MAX_K (beyond: status 9), whatever
+ * the kernel; integers of -128 are fine.  Results are computed in fp32 and rounded once to c_type.  act as in
+ * ppml_b200_mul_mat_f32_fused; bias (fp32) and gate (c_type) may be NULL.  Every matrix has a row pitch in elements (ld_*,
+ * >= its row length; elements behind a row are neither read into results nor written).
+ * quantize_tokens_i8 serves weights too: a row of W is an output channel.
+ * path: AUTO / UMMA use the tensor cores where A and B are 16-byte aligned with pitches that are multiples of 16 bytes
+ * (UMMA: status 7 otherwise), SIMT the CUDA cores; the sums are the same, so the results agree bit for bit for act = 0.
+ * linear_i8 quantizes X on the way.  workspace: device memory of ppml_b200_linear_i8_workspace(M, K) bytes, 16-byte aligned,
+ * used on `stream` only while the call runs there.  M = 0 is a call without work (status 0). */
+#define PPML_B200_TYPE_F32 0
+#define PPML_B200_TYPE_F16 1
+#define PPML_B200_TYPE_BF16 2
+#define PPML_B200_I8_MAX_K 131071
+int ppml_b200_quantize_tokens_i8(const void* x, int x_type, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int64_t M, int K,
+                                 void* stream);
+int ppml_b200_mul_mat_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb, const float* b_scale,
+                         void* C, int64_t ldc, int c_type, int M, int K, int N, const float* bias, const void* gate, int64_t ld_gate,
+                         int act, int path, void* stream);
+int64_t ppml_b200_linear_i8_workspace(int64_t M, int K);
+int ppml_b200_linear_i8(const void* X, int x_type, int64_t ld_x, const int8_t* B, int64_t ldb, const float* b_scale, void* C,
+                        int64_t ldc, int c_type, int M, int K, int N, const float* bias, const void* gate, int64_t ld_gate, int act,
+                        int path, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- Q8_0 weights on disk --------------------------------------------------------------------
  * No counterpart in the reference, which refuses to save quantized tensors (src/model/GGUF.cpp:204-213) and
  * re-quantizes on the host at every start (src/model/PPML.cpp:4504-4524).  The container is the reference's
@@ -238,6 +267,51 @@ int ppml_b200_flash_attn_forward_tokens(const ppml_b200_flash_cfg* cfg, int Lk, 
                                         const float* Q, const float* K, const float* V, int64_t ld_q, int64_t ld_kv,
                                         const float* bias, const float* gate, int64_t ld_gate, int act, float* O, int64_t ld_o,
                                         float* LSE, int path, void* stream);
+
+/* ---- norms of queries and keys for each head, with the position rotation --------------------------------------------
+ * What stands between the Q / K projections and the attention entries above in models that normalise each head and encode
+ * positions by rotation; no counterpart in the reference (its position encodings are added to the activations).  One pass
+ * over Q and K, in place or into the layout that the attention reads:
+ *   xhat = (x - mu) / sqrt(mean((x - mu)^2) + eps) over the d values of one head of one token; mu = 0 for norm 1 (root mean
+ *          square), the mean for norm 2 (LayerNorm without bias); xhat = x for norm 0
+ *   n    = xhat * weight    (q_weight / k_weight [d] fp32, shared by the heads of Q / of K; NULL: 1)
+ *   y    = n with the first `rot` dims rotated by the token's row of the table: (a, b) -> (a cos - b sin, b cos + a sin) for the
+ *          pairs (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved = 1; the other dims pass.
+ * cos / sin: [table_rows][rot / 2] fp32.  positions (int32): row of the table per token, [B][L] with batch stride pos_b (0: one
+ * [L] for every batch); NULL: token l of a batch is at position l (L <= table_rows).  A token with a negative position is
+ * padding: its results are left as they were, its input gradients are 0, and it adds nothing to the weight gradients.  A
+ * position beyond the table is never looked up: the token's rotated results (and gradients) are NaN.
+ * Views: element (b, l, h, i) at p[b * sb + l * sl + h * sh + i]; Q, K and results may be strided in any way (ranges of a fused
+ * projection, [B][L][h][d], [B][h][L][d]), inputs also with stride 0; elements of a result must lie apart (status 1), and a
+ * result may be its own input's memory with the same strides.  hq and hk may
+ * differ; one of them may be 0 (its views NULL).  d up to 512 (beyond: status 9), B * L below 2^31.
+ * The backward pass takes the forward's inputs and the results' gradients dQo, dKo and writes dQ, dK (both sides, all of it) and,
+ * where the pointers are given, dq_weight / dk_weight [d] fp32 (they are overwritten, and summed in a fixed order).  Those need a
+ * workspace of ppml_b200_qk_norm_rope_backward_workspace(cfg) bytes, 16-byte aligned, used on `stream` only while the call
+ * runs there (NULL when neither is wanted).  Math in fp32, one rounding to `type` (PPML_B200_TYPE_*) where a result is stored. */
+typedef struct ppml_b200_qk_cfg {
+    int B, L, hq, hk, d;
+    int type;
+    int norm;                 /* 0 none, 1 root mean square, 2 LayerNorm */
+    float eps;
+    int rot;                  /* even, 0 .. d */
+    int interleaved;
+    int table_rows;
+    int64_t pos_b;
+} ppml_b200_qk_cfg;
+typedef struct ppml_b200_heads {
+    void* p;
+    int64_t sb, sl, sh;       /* elements */
+} ppml_b200_heads;
+int ppml_b200_qk_norm_rope(const ppml_b200_qk_cfg* cfg, const ppml_b200_heads* Q, const ppml_b200_heads* K, const float* q_weight,
+                           const float* k_weight, const float* cos, const float* sin, const int32_t* positions,
+                           const ppml_b200_heads* Qo, const ppml_b200_heads* Ko, void* stream);
+int64_t ppml_b200_qk_norm_rope_backward_workspace(const ppml_b200_qk_cfg* cfg);
+int ppml_b200_qk_norm_rope_backward(const ppml_b200_qk_cfg* cfg, const ppml_b200_heads* Q, const ppml_b200_heads* K,
+                                    const float* q_weight, const float* k_weight, const float* cos, const float* sin,
+                                    const int32_t* positions, const ppml_b200_heads* dQo, const ppml_b200_heads* dKo,
+                                    const ppml_b200_heads* dQ, const ppml_b200_heads* dK, float* dq_weight, float* dk_weight,
+                                    void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- OP_OUT_PROD -------------------------------------------------------------------------------
  * Replaces out_prod_cuda (src/backend/CUDAKernels.cpp:201; src/cuda/OutProdKernel.cu:211-260):

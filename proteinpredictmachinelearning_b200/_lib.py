@@ -8,12 +8,23 @@ LIB_PATH = os.path.join(_HERE, "lib", "libppml_b200.so")
 
 PATH_AUTO, PATH_SIMT, PATH_UMMA = 0, 1, 2
 TF32_ROUND, TF32_TMA, TF32_TRUNCATE = 0, 1, 2
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+I8_MAX_K = 131071                    # PPML_B200_I8_MAX_K
 NOALLOC_SCRATCH_BYTES = 4 << 20      # PPML_B200_NOALLOC_SCRATCH_BYTES
 
 
 class FlashCfg(C.Structure):
     _fields_ = [("B", C.c_int), ("h", C.c_int), ("L", C.c_int), ("d", C.c_int), ("causal", C.c_int),
                 ("scale", C.c_float), ("softmax_eps", C.c_float), ("Br", C.c_int), ("Bc", C.c_int)]
+
+
+class QkCfg(C.Structure):
+    _fields_ = [("B", C.c_int), ("L", C.c_int), ("hq", C.c_int), ("hk", C.c_int), ("d", C.c_int), ("type", C.c_int), ("norm", C.c_int),
+                ("eps", C.c_float), ("rot", C.c_int), ("interleaved", C.c_int), ("table_rows", C.c_int), ("pos_b", C.c_int64)]
+
+
+class Heads(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("sb", C.c_int64), ("sl", C.c_int64), ("sh", C.c_int64)]
 
 
 _vp, _i, _i64, _f = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -35,6 +46,14 @@ SIGNATURES = {
     "ppml_b200_cast_f32_to_bf16": (_i, [_vp, _vp, _i64, _vp]),
     "ppml_b200_mul_mat_q8": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, C.POINTER(_i), _vp]),
     "ppml_b200_mul_mat_q8_noalloc": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "ppml_b200_quantize_tokens_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _i64, _i, _vp]),
+    "ppml_b200_mul_mat_i8": (_i, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp]),
+    "ppml_b200_linear_i8_workspace": (_i64, [_i64, _i]),
+    "ppml_b200_linear_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp, _i64, _vp]),
+    "ppml_b200_qk_norm_rope": (_i, [C.POINTER(QkCfg), C.POINTER(Heads), C.POINTER(Heads)] + [_vp] * 5 + [C.POINTER(Heads)] * 2 + [_vp]),
+    "ppml_b200_qk_norm_rope_backward_workspace": (_i64, [C.POINTER(QkCfg)]),
+    "ppml_b200_qk_norm_rope_backward": (_i, [C.POINTER(QkCfg), C.POINTER(Heads), C.POINTER(Heads)] + [_vp] * 5 + [C.POINTER(Heads)] * 4 +
+                                        [_vp, _vp, _vp, _i64, _vp]),
     "ppml_b200_quantize_rows_q8_1": (_i, [_vp, _vp, _i64, _vp]),
     "ppml_b200_dequantize_q8_0": (_i, [_vp, _vp, _i64, _vp]),
     "ppml_b200_dequantize_q8_1": (_i, [_vp, _vp, _i64, _vp]),

@@ -10,6 +10,7 @@
 #include <mutex>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "../../include/ppml_b200.h"
@@ -283,6 +284,158 @@ int ppml_b200_quantize_q8_0r(const float* w_dev, void* q8_0r_dev, int64_t ne, vo
 int64_t ppml_b200_q8_0r_bytes(int64_t numel) { return numel / 32 * 34; }
 int ppml_b200_repack_q8_0(const void* blocks34_dev, int64_t nblocks, void* q8_0r_dev, void* stream) {
     return launch_repack_q8_0(blocks34_dev, nblocks, q8_0r_dev, as_stream(stream));
+}
+
+// ---- 8-bit integers with a scale per token and per output channel ----
+namespace {
+inline bool type_ok(int t) { return t >= kTypeF32 && t <= kTypeBF16; }
+inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+inline uintptr_t type_bytes(int t) { return t == kTypeF32 ? 4 : 2; }
+constexpr int64_t round16(int64_t v) { return (v + 15) & ~static_cast<int64_t>(15); }
+
+// The checks that both product entries share (their integer operand A aside).
+int check_i8(const int8_t* B, int64_t ldb, const float* b_scale, const void* C, int64_t ldc, int c_type, int M, int K, int N,
+             const void* gate, int64_t ld_gate, int act, int path) {
+    if (M < 0 || K <= 0 || N <= 0 || act < 0 || act > 5 || !path_ok(path) || !type_ok(c_type)) return ST_BAD_ARGS;
+    if (K > kI8MaxK) return ST_TOO_LARGE;
+    if (!B || !b_scale || ldb < K || ldc < N || (gate && ld_gate < N) || !aligned(b_scale, 4)) return ST_BAD_ARGS;
+    if (M > 0 && (!C || !aligned(C, type_bytes(c_type)) || !aligned(gate, type_bytes(c_type)))) return ST_BAD_ARGS;
+    return ST_OK;
+}
+int i8_product(const I8Product& p, int path, cudaStream_t st) {
+    if (path == PPML_B200_PATH_UMMA) return ST_UNSUPPORTED_PATH;
+    return launch_i8_dp4a(p, st);
+}
+}  // namespace
+
+int ppml_b200_quantize_tokens_i8(const void* x, int x_type, int64_t ld_x, int8_t* q, int64_t ld_q, float* scale, int64_t M, int K,
+                                 void* stream) {
+    if (M < 0 || M > INT32_MAX || K <= 0 || !type_ok(x_type) || ld_x < K || ld_q < K) return ST_BAD_ARGS;
+    if (M == 0) return ST_OK;
+    if (!x || !q || !scale || !aligned(x, type_bytes(x_type)) || !aligned(scale, 4)) return ST_BAD_ARGS;
+    return launch_quantize_tokens(x, x_type, ld_x, q, ld_q, scale, M, K, as_stream(stream));
+}
+
+int ppml_b200_mul_mat_i8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb, const float* b_scale,
+                         void* C, int64_t ldc, int c_type, int M, int K, int N, const float* bias, const void* gate, int64_t ld_gate,
+                         int act, int path, void* stream) {
+    const int bad = check_i8(B, ldb, b_scale, C, ldc, c_type, M, K, N, gate, ld_gate, act, path);
+    if (bad != ST_OK) return bad;
+    if (lda < K || !aligned(bias, 4)) return ST_BAD_ARGS;
+    if (M == 0) return ST_OK;
+    if (!A || !a_scale || !aligned(a_scale, 4)) return ST_BAD_ARGS;
+    const I8Product p{A, B, lda, ldb, a_scale, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act};
+    return i8_product(p, path, as_stream(stream));
+}
+
+int64_t ppml_b200_linear_i8_workspace(int64_t M, int K) {
+    return M <= 0 || K <= 0 ? 0 : M * round16(K) + round16(4 * M);
+}
+
+int ppml_b200_linear_i8(const void* X, int x_type, int64_t ld_x, const int8_t* B, int64_t ldb, const float* b_scale, void* C,
+                        int64_t ldc, int c_type, int M, int K, int N, const float* bias, const void* gate, int64_t ld_gate, int act,
+                        int path, void* workspace, int64_t workspace_bytes, void* stream) {
+    const int bad = check_i8(B, ldb, b_scale, C, ldc, c_type, M, K, N, gate, ld_gate, act, path);
+    if (bad != ST_OK) return bad;
+    if (!type_ok(x_type) || ld_x < K || !aligned(bias, 4)) return ST_BAD_ARGS;
+    if (M == 0) return ST_OK;
+    if (!X || !aligned(X, type_bytes(x_type))) return ST_BAD_ARGS;
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < ppml_b200_linear_i8_workspace(M, K)) return ST_SCRATCH;
+    int8_t* q = static_cast<int8_t*>(workspace);
+    const int64_t ld = round16(K);
+    float* scale = reinterpret_cast<float*>(q + M * ld);
+    const int rc = launch_quantize_tokens(X, x_type, ld_x, q, ld, scale, M, K, as_stream(stream));
+    if (rc != ST_OK) return rc;
+    const I8Product p{q, B, ld, ldb, scale, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act};
+    return i8_product(p, path, as_stream(stream));
+}
+
+// ---- per-head norms of Q and K with the position rotation ----
+namespace {
+bool view_ok(const ppml_b200_heads* v, int heads, uintptr_t elem) {
+    if (heads == 0) return true;
+    return v && v->p && aligned(v->p, elem) && v->sb >= 0 && v->sl >= 0 && v->sh >= 0;
+}
+// Whether no two elements of a result share memory: each stride covers what the smaller ones span.
+bool view_apart(const ppml_b200_heads* v, const ppml_b200_qk_cfg* c, int heads) {
+    if (heads == 0) return true;
+    int64_t stride[3] = {v->sb, v->sl, v->sh}, n[3] = {c->B, c->L, heads};
+    for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2 - i; ++j)
+            if (stride[j] > stride[j + 1]) { std::swap(stride[j], stride[j + 1]); std::swap(n[j], n[j + 1]); }
+    int64_t span = c->d;
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] == 1) continue;
+        if (stride[i] < span) return false;
+        if (stride[i] > (INT64_MAX - span) / n[i]) return false;
+        span += stride[i] * (n[i] - 1);
+    }
+    return true;
+}
+// The argument checks of both directions; fills what they share.  ST_OK with out->B == 0: nothing to do.
+int qk_params(const ppml_b200_qk_cfg* c, const ppml_b200_heads* Q, const ppml_b200_heads* K, const float* qw, const float* kw,
+              const float* cos_t, const float* sin_t, const int32_t* positions, const ppml_b200_heads* Qo, const ppml_b200_heads* Ko,
+              QkParams* out) {
+    if (!c || c->B < 0 || c->L < 0 || c->hq < 0 || c->hk < 0 || c->hq > INT32_MAX - c->hk || c->hq + c->hk == 0 || c->d <= 0 ||
+        !type_ok(c->type) || c->norm < 0 || c->norm > 2 || c->rot < 0 || c->rot > c->d || c->rot % 2 != 0 || !(c->eps >= 0.0f))
+        return ST_BAD_ARGS;
+    if (c->d > kQkMaxDim || static_cast<int64_t>(c->B) * c->L > INT32_MAX) return ST_TOO_LARGE;
+    *out = QkParams{};
+    if (c->B == 0 || c->L == 0) return ST_OK;
+    const uintptr_t e = type_bytes(c->type);
+    if (!view_ok(Q, c->hq, e) || !view_ok(K, c->hk, e) || !view_ok(Qo, c->hq, e) || !view_ok(Ko, c->hk, e)) return ST_BAD_ARGS;
+    if (!aligned(qw, 4) || !aligned(kw, 4) || !aligned(cos_t, 4) || !aligned(sin_t, 4) || !aligned(positions, 4)) return ST_BAD_ARGS;
+    if (c->rot > 0 && (!cos_t || !sin_t || c->table_rows <= 0)) return ST_BAD_ARGS;
+    if (positions ? c->pos_b < 0 : (c->rot > 0 && c->L > c->table_rows)) return ST_BAD_ARGS;
+    auto view = [](const ppml_b200_heads* v, int heads) { return heads ? HeadsView{v->p, v->sb, v->sl, v->sh} : HeadsView{}; };
+    out->q = view(Q, c->hq); out->k = view(K, c->hk); out->qo = view(Qo, c->hq); out->ko = view(Ko, c->hk);
+    out->qw = qw; out->kw = kw; out->cos_t = cos_t; out->sin_t = sin_t; out->positions = positions; out->pos_b = c->pos_b;
+    out->B = c->B; out->L = c->L; out->hq = c->hq; out->hk = c->hk; out->d = c->d; out->norm = c->norm; out->rot = c->rot;
+    out->interleaved = c->interleaved ? 1 : 0; out->table_rows = c->table_rows; out->eps = c->eps;
+    return ST_OK;
+}
+}  // namespace
+
+int ppml_b200_qk_norm_rope(const ppml_b200_qk_cfg* cfg, const ppml_b200_heads* Q, const ppml_b200_heads* K, const float* q_weight,
+                           const float* k_weight, const float* cos, const float* sin, const int32_t* positions,
+                           const ppml_b200_heads* Qo, const ppml_b200_heads* Ko, void* stream) {
+    QkParams p;
+    const int rc = qk_params(cfg, Q, K, q_weight, k_weight, cos, sin, positions, Qo, Ko, &p);
+    if (rc != ST_OK || p.B == 0) return rc;
+    if (!view_apart(Qo, cfg, cfg->hq) || !view_apart(Ko, cfg, cfg->hk)) return ST_BAD_ARGS;
+    return launch_qk_norm_rope(p, cfg->type, false, as_stream(stream));
+}
+
+int64_t ppml_b200_qk_norm_rope_backward_workspace(const ppml_b200_qk_cfg* cfg) {
+    if (!cfg || cfg->d <= 0 || cfg->d > kQkMaxDim) return 0;
+    return static_cast<int64_t>(kQkMaxBlocks) * 2 * cfg->d * static_cast<int64_t>(sizeof(float));
+}
+
+int ppml_b200_qk_norm_rope_backward(const ppml_b200_qk_cfg* cfg, const ppml_b200_heads* Q, const ppml_b200_heads* K,
+                                    const float* q_weight, const float* k_weight, const float* cos, const float* sin,
+                                    const int32_t* positions, const ppml_b200_heads* dQo, const ppml_b200_heads* dKo,
+                                    const ppml_b200_heads* dQ, const ppml_b200_heads* dK, float* dq_weight, float* dk_weight,
+                                    void* workspace, int64_t workspace_bytes, void* stream) {
+    QkParams p;
+    const int rc = qk_params(cfg, Q, K, q_weight, k_weight, cos, sin, positions, dQo, dKo, &p);
+    if (rc != ST_OK) return rc;
+    const uintptr_t e = type_bytes(cfg->type);
+    cudaStream_t st = as_stream(stream);
+    if (!aligned(dq_weight, 4) || !aligned(dk_weight, 4)) return ST_BAD_ARGS;
+    if (p.B == 0) {                                // no tokens: the weight gradients are sums over nothing
+        for (float* w : {dq_weight, dk_weight})
+            if (w && cudaMemsetAsync(w, 0, cfg->d * sizeof(float), st) != cudaSuccess) return ST_LAUNCH;
+        return ST_OK;
+    }
+    if (!view_ok(dQ, cfg->hq, e) || !view_ok(dK, cfg->hk, e)) return ST_BAD_ARGS;
+    if (!view_apart(dQ, cfg, cfg->hq) || !view_apart(dK, cfg, cfg->hk)) return ST_BAD_ARGS;
+    if (cfg->hq) p.dq = HeadsView{dQ->p, dQ->sb, dQ->sl, dQ->sh};
+    if (cfg->hk) p.dk = HeadsView{dK->p, dK->sb, dK->sl, dK->sh};
+    if (dq_weight || dk_weight) {
+        if (!workspace || !aligned(workspace, 16) || workspace_bytes < ppml_b200_qk_norm_rope_backward_workspace(cfg)) return ST_SCRATCH;
+        p.partial = static_cast<float*>(workspace); p.dqw = dq_weight; p.dkw = dk_weight;
+    }
+    return launch_qk_norm_rope(p, cfg->type, true, st);
 }
 
 namespace {

@@ -1,0 +1,105 @@
+// i8_simt.cu -- 8-bit integers with a scale per token and per output channel on CUDA cores: the token quantizer, and the
+// product for operands that TMA cannot address (a row pitch or a base off 16 bytes) and for PATH_SIMT.
+#include "i8_common.cuh"
+
+namespace ppml_b200 {
+namespace {
+
+// One block per row; the second pass over the row comes from L1 / L2.
+template <typename T>
+__global__ void __launch_bounds__(128) quantize_tokens_kernel(const T* __restrict__ x, long long ld_x, int8_t* __restrict__ q, long long ld_q,
+                                                              float* __restrict__ scale, int K) {
+    __shared__ uint32_t part[4];
+    const long long row = blockIdx.x;
+    const T* xr = x + row * ld_x;
+    uint32_t top = 0;
+    for (int k = threadIdx.x; k < K; k += 128) top = max(top, magnitude_bits(to_f32(xr[k])));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+    __syncthreads();
+    const float s = i8_scale(max(max(part[0], part[1]), max(part[2], part[3])));
+    int8_t* qr = q + row * ld_q;
+    for (int k = threadIdx.x; k < K; k += 128) qr[k] = static_cast<int8_t>(i8_quantize(to_f32(xr[k]), s));
+    if (threadIdx.x == 0) scale[row] = s;
+}
+
+// 64 x 64 outputs per block of 256 threads, 4 x 4 each; 64 k per step as 16 words of four, dp4a.  Rows that are not 4-byte
+// aligned are read byte by byte.
+constexpr int kT = 64, kWords = 16;
+
+__device__ __forceinline__ int load_word(const int8_t* row, int k, int K, bool aligned) {
+    if (aligned && k + 4 <= K) return *reinterpret_cast<const int*>(row + k);
+    uint32_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (k + i < K) v |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * i);
+    return static_cast<int>(v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) i8_dp4a_kernel(I8Product p) {
+    __shared__ int As[kWords][kT + 1], Bs[kWords][kT + 1];
+    const long long m0 = static_cast<long long>(blockIdx.x) * kT, n0 = static_cast<long long>(blockIdx.y) * kT;
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const bool a_al = ((reinterpret_cast<uintptr_t>(p.A) | p.lda) & 3) == 0, b_al = ((reinterpret_cast<uintptr_t>(p.B) | p.ldb) & 3) == 0;
+    int acc[4][4] = {};
+    for (int k0 = 0; k0 < p.K; k0 += 4 * kWords) {
+        for (int i = threadIdx.x; i < kT * kWords; i += 256) {
+            const int w = i & (kWords - 1), r = i >> 4;
+            As[w][r] = m0 + r < p.M ? load_word(p.A + (m0 + r) * p.lda, k0 + 4 * w, p.K, a_al) : 0;
+            Bs[w][r] = n0 + r < p.N ? load_word(p.B + (n0 + r) * p.ldb, k0 + 4 * w, p.K, b_al) : 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWords; ++w) {
+            int a[4], b[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { a[i] = As[w][ty + 16 * i]; b[i] = Bs[w][tx + 16 * i]; }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(a[i], b[j], acc[i][j]);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long m = m0 + ty + 16 * i;
+        if (m >= p.M) continue;
+        const float sa = p.a_scale[m];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const long long n = n0 + tx + 16 * j;
+            if (n >= p.N) continue;
+            float y = i8_epilogue(acc[i][j], sa, p.b_scale[n], p.bias ? p.bias[n] : 0.0f, p.act);
+            if (p.gate) y *= to_f32(static_cast<const T*>(p.gate)[m * p.ld_gate + n]);
+            static_cast<T*>(p.C)[m * p.ldc + n] = from_f32<T>(y);
+        }
+    }
+}
+
+}  // namespace
+
+int launch_quantize_tokens(const void* x, int type, long long ld_x, int8_t* q, long long ld_q, float* scale, long long rows, int K,
+                           cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(rows));
+    switch (type) {
+        case kTypeF32: quantize_tokens_kernel<float><<<grid, 128, 0, st>>>(static_cast<const float*>(x), ld_x, q, ld_q, scale, K); break;
+        case kTypeF16: quantize_tokens_kernel<__half><<<grid, 128, 0, st>>>(static_cast<const __half*>(x), ld_x, q, ld_q, scale, K); break;
+        default: quantize_tokens_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ld_x, q, ld_q, scale, K);
+    }
+    return cudaGetLastError() == cudaSuccess ? ST_OK : ST_LAUNCH;
+}
+
+int launch_i8_dp4a(const I8Product& p, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>((p.M + static_cast<long long>(kT) - 1) / kT), static_cast<unsigned>((p.N + static_cast<long long>(kT) - 1) / kT));
+    if (grid.y > 65535u) return ST_TOO_LARGE;
+    switch (p.c_type) {
+        case kTypeF32: i8_dp4a_kernel<float><<<grid, 256, 0, st>>>(p); break;
+        case kTypeF16: i8_dp4a_kernel<__half><<<grid, 256, 0, st>>>(p); break;
+        default: i8_dp4a_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+    }
+    return cudaGetLastError() == cudaSuccess ? ST_OK : ST_LAUNCH;
+}
+
+}  // namespace ppml_b200

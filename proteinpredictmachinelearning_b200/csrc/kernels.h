@@ -118,6 +118,39 @@ int launch_umma_attn(const void* Q, const void* K, const void* V, int elem, cons
                      int B, int H, int L, int Lk, int d, int causal, float scale, float eps,
                      long long bias_batch_stride, int ft, const AttnLayout& lay, cudaStream_t st);
 
+// Element types of the entries that take more than one (PPML_B200_TYPE_*).
+enum : int { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2 };
+
+// 8-bit integers with a scale per token and per output channel (i8_simt.cu).
+constexpr int kI8MaxK = 131071;        // 128 * 128 * K stays inside int32
+struct I8Product {
+    const int8_t* A; const int8_t* B;  // [M][K], [N][K] with row pitches lda, ldb
+    long long lda, ldb;
+    const float* a_scale; const float* b_scale; const float* bias;
+    void* C; const void* gate;         // [M][N] of c_type with pitches ldc, ld_gate; gate may be null
+    long long ldc, ld_gate;
+    int M, N, K, c_type, act;
+};
+int launch_quantize_tokens(const void* x, int type, long long ld_x, int8_t* q, long long ld_q, float* scale, long long rows, int K,
+                           cudaStream_t st);
+int launch_i8_dp4a(const I8Product& p, cudaStream_t st);
+
+// Per-head norms of Q and K with the position rotation (qk_norm_rope.cu).  Element (b, l, h, i) of a view is at
+// p[b * b_stride + l * l_stride + h * h_stride + i].
+struct HeadsView { void* p; long long b, l, h; };
+constexpr int kQkMaxDim = 512;
+constexpr int kQkMaxBlocks = 1184;     // lines of the weight gradients' workspace
+struct QkParams {
+    HeadsView q, k, qo, ko, dq, dk;    // backward: qo, ko hold the gradients of the results
+    const float* qw; const float* kw; const float* cos_t; const float* sin_t; const int* positions;
+    float* dqw; float* dkw; float* partial;
+    long long pos_b;
+    int B, L, hq, hk, d, norm, rot, interleaved, table_rows;
+    float eps;
+};
+unsigned qk_blocks(long long rows);
+int launch_qk_norm_rope(const QkParams& p, int type, bool backward, cudaStream_t st);
+
 int num_sms();
 
 }  // namespace ppml_b200
