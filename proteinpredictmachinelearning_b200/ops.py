@@ -185,86 +185,128 @@ def mul_mat_q8_noalloc(W, X, M, wtype=2, c_trans=1, bias=None, out=None):
 
 TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
 
-
-def _require(cond, what):
-    if not cond:
-        raise ValueError(what)
-
-
-def _rows(t, dtype, shape, device, name):
-    """A matrix whose rows are contiguous: its row pitch in elements."""
-    _require(t.is_cuda and t.device == device, f"{name} must be on {device}")
-    _require(t.dtype in (dtype if isinstance(dtype, tuple) else (dtype,)), f"{name}: type {t.dtype}")
-    _require(tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(t.shape)}, {tuple(shape)} is wanted")
-    if t.shape[0] <= 1:
-        _require(t.shape[1] <= 1 or t.stride(1) == 1, f"{name}: rows must be contiguous")
-        return max(t.shape[1], t.stride(0))
-    _require((t.shape[1] <= 1 or t.stride(1) == 1) and t.stride(0) >= t.shape[1], f"{name}: rows must be contiguous and apart")
-    return t.stride(0)
+# The entries from here to qk_norm_rope_backward are called many times for a token, so their host side is kept short: pointers go to
+# the library as plain integers, messages are only put together for a refusal, and the device is only switched when the
+# tensors' is not the current one.
 
 
-def _vector(t, n, device, name):
-    if t is not None:
-        _require(t.is_cuda and t.device == device and t.dtype == torch.float32 and tuple(t.shape) == (n,) and t.is_contiguous(),
-                 f"{name}: {n} contiguous fp32 values on {device} are wanted")
-    return _p(t)
+def _on(device):
+    """Context for a launch on the tensors' device; None when that is the current one."""
+    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _raw_stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index) or None
+
+
+def _refuse(name, t, want):
+    raise ValueError(f"{name}: {want} wanted, got {tuple(t.shape)} of {t.dtype} on {t.device} with strides {t.stride()}")
+
+
+def _pitch(t, dtype, M, K, device, name):
+    """The row pitch of a matrix whose rows are contiguous and lie apart."""
+    shape = t.shape
+    if len(shape) == 2 and shape[0] == M and shape[1] == K and t.dtype == dtype and t.device == device:
+        s0, s1 = t.stride()
+        if s1 == 1 or K <= 1:
+            if M <= 1:
+                return s0 if s0 > K else K
+            if s0 >= K:
+                return s0
+    _refuse(name, t, f"[{M}, {K}] of {dtype} on {device}, rows contiguous and apart,")
+
+
+def _vec(t, n, device, name):
+    """The address of n contiguous fp32 values; None for None."""
+    if t is None:
+        return None
+    if t.dtype == torch.float32 and t.device == device and t.shape == (n,) and (n <= 1 or t.stride(0) == 1):
+        return t.data_ptr()
+    _refuse(name, t, f"{n} contiguous fp32 values on {device}")
+
+
+def _matrix(x, name):
+    if x.dim() != 2 or not x.is_cuda or x.dtype not in TYPE:
+        _refuse(name, x, "a matrix of fp32, fp16 or bf16 on the GPU")
 
 
 def quantize_tokens_i8(x, out=None):
     """x [M, K] (fp32, fp16 or bf16; rows contiguous, any pitch) -> (int8 [M, K], fp32 scales [M]): scale = max |x| / 127 of the
     row, q = round(x / scale).  New integers get a row pitch that is a multiple of 16 bytes, which the tensor-core product
     wants.  Weights [N, K] are quantized the same way, one scale for each output channel."""
-    _require(x.dim() == 2 and x.is_cuda and x.dtype in TYPE, "x: a matrix of fp32, fp16 or bf16 on the GPU is wanted")
+    _matrix(x, "x")
     M, K = x.shape
-    ld = _rows(x, x.dtype, (M, K), x.device, "x")
-    with torch.cuda.device(x.device):
-        if out is None:
-            out = (torch.empty((M, (K + 15) // 16 * 16), device=x.device, dtype=torch.int8)[:, :K], torch.empty(M, device=x.device))
-        q, scale = out
-        rc = _lib.load().ppml_b200_quantize_tokens_i8(_p(x), TYPE[x.dtype], ld, _p(q), _rows(q, torch.int8, (M, K), x.device, "q"),
-                                                      _vector(scale, M, x.device, "scale"), M, K, _stream())
-    _check(rc, "quantize_tokens_i8")
-    return q, scale
-
-
-def _i8_operands(device, M, K, W, w_scale, bias, gate, act, dtype, out):
-    """What both products check alike: (N, the output, the arguments from B to ldc, those from bias to act)."""
-    _require(W.dim() == 2 and dtype in TYPE and act in ACT, "mul_mat_i8: a weight matrix, a floating type and a known act are wanted")
-    N = W.shape[0]
-    ldb = _rows(W, torch.int8, (N, K), device, "W")
-    scale = _vector(w_scale, N, device, "w_scale")
+    dev = x.device
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return quantize_tokens_i8(x, out)
+    ld = _pitch(x, x.dtype, M, K, dev, "x")
     if out is None:
-        out = torch.empty((M, N), device=device, dtype=dtype)
-    ldc = _rows(out, dtype, (M, N), device, "out")
-    ldg = 0 if gate is None else _rows(gate, dtype, (M, N), device, "gate")
-    return N, out, (_p(W), ldb, scale, _p(out), ldc, TYPE[dtype]), (_vector(bias, N, device, "bias"), _p(gate), ldg, ACT[act])
+        q = torch.empty((M, (K + 15) & -16), device=dev, dtype=torch.int8)
+        out = (q if q.shape[1] == K else q[:, :K], torch.empty(M, device=dev, dtype=torch.float32))
+    q, scale = out
+    rc = _lib.load().ppml_b200_quantize_tokens_i8(x.data_ptr(), TYPE[x.dtype], ld, q.data_ptr(), _pitch(q, torch.int8, M, K, dev, "q"),
+                                                  _vec(scale, M, dev, "scale"), M, K, _raw_stream(dev))
+    if rc:
+        _check(rc, "quantize_tokens_i8")
+    return out
+
+
+def _product_args(dev, M, K, W, w_scale, bias, gate, act, dtype, path, out):
+    """What both products check and pass alike: the output, the arguments from B to path."""
+    if W.dim() != 2:
+        _refuse("W", W, f"[N, {K}]")
+    if act not in ACT or dtype not in TYPE:
+        raise ValueError(f"act: one of {sorted(ACT)}; type: fp32, fp16 or bf16; got {act!r}, {dtype}")
+    N = W.shape[0]
+    ldb = _pitch(W, torch.int8, N, K, dev, "W")
+    if out is None:
+        out, ldc = torch.empty((M, N), device=dev, dtype=dtype), N
+    else:
+        ldc = _pitch(out, dtype, M, N, dev, "out")
+    g, ldg = (None, 0) if gate is None else (gate.data_ptr(), _pitch(gate, dtype, M, N, dev, "gate"))
+    return out, (W.data_ptr(), ldb, _vec(w_scale, N, dev, "w_scale"), out.data_ptr(), ldc, TYPE[dtype], M, K, N,
+                 _vec(bias, N, dev, "bias"), g, ldg, ACT[act], path)
 
 
 def mul_mat_i8(A, a_scale, W, w_scale, bias=None, gate=None, act="none", dtype=torch.float32, path=PATH_AUTO, out=None):
     """act(a_scale[m] * w_scale[n] * sum_k A[m, k] W[n, k] + bias[n]) * gate[m, n]: A int8 [M, K] and W int8 [N, K] with their
     scales (quantize_tokens_i8), exact int32 sums, fp32 behind them, one rounding to `dtype` (of out and gate)."""
-    _require(A.dim() == 2 and A.is_cuda, "A: an int8 matrix on the GPU is wanted")
+    if A.dim() != 2 or not A.is_cuda:
+        _refuse("A", A, "an int8 matrix on the GPU")
     M, K = A.shape
-    with torch.cuda.device(A.device):
-        lda = _rows(A, torch.int8, (M, K), A.device, "A")
-        N, out, head, tail = _i8_operands(A.device, M, K, W, w_scale, bias, gate, act, dtype if out is None else out.dtype, out)
-        rc = _lib.load().ppml_b200_mul_mat_i8(_p(A), lda, _vector(a_scale, M, A.device, "a_scale"), *head, M, K, N, *tail, path, _stream())
-    _check(rc, "mul_mat_i8")
+    dev = A.device
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return mul_mat_i8(A, a_scale, W, w_scale, bias, gate, act, dtype, path, out)
+    lda = _pitch(A, torch.int8, M, K, dev, "A")
+    out, args = _product_args(dev, M, K, W, w_scale, bias, gate, act, dtype if out is None else out.dtype, path, out)
+    rc = _lib.load().ppml_b200_mul_mat_i8(A.data_ptr(), lda, _vec(a_scale, M, dev, "a_scale"), *args, _raw_stream(dev))
+    if rc:
+        _check(rc, "mul_mat_i8")
     return out
 
 
 def linear_i8(x, W, w_scale, bias=None, gate=None, act="none", dtype=None, path=PATH_AUTO, out=None):
     """quantize_tokens_i8 and mul_mat_i8 as one call: x [M, K] fp32, fp16 or bf16; the result has x's type unless `dtype` (or
     `out`) says otherwise."""
-    _require(x.dim() == 2 and x.is_cuda and x.dtype in TYPE, "x: a matrix of fp32, fp16 or bf16 on the GPU is wanted")
+    _matrix(x, "x")
     M, K = x.shape
+    dev = x.device
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return linear_i8(x, W, w_scale, bias, gate, act, dtype, path, out)
     lib = _lib.load()
-    with torch.cuda.device(x.device):
-        ld = _rows(x, x.dtype, (M, K), x.device, "x")
-        N, out, head, tail = _i8_operands(x.device, M, K, W, w_scale, bias, gate, act, out.dtype if out is not None else dtype or x.dtype, out)
-        ws = torch.empty(lib.ppml_b200_linear_i8_workspace(M, K), device=x.device, dtype=torch.uint8)
-        rc = lib.ppml_b200_linear_i8(_p(x), TYPE[x.dtype], ld, *head, M, K, N, *tail, path, _p(ws), ws.numel(), _stream())
-    _check(rc, "linear_i8")
+    ld = _pitch(x, x.dtype, M, K, dev, "x")
+    out, args = _product_args(dev, M, K, W, w_scale, bias, gate, act, out.dtype if out is not None else dtype or x.dtype, path, out)
+    need = lib.ppml_b200_linear_i8_workspace(M, K)
+    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    rc = lib.ppml_b200_linear_i8(x.data_ptr(), TYPE[x.dtype], ld, *args, None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
+    if rc:
+        _check(rc, "linear_i8")
     return out
 
 
@@ -273,47 +315,57 @@ NORM = {"none": 0, "rms": 1, "layer": 2}
 
 def rope_table(rows, rot, base=10000.0, device="cuda"):
     """cos and sin [rows, rot / 2] fp32 of position * base^(-2 i / rot), the angles in 64 bits."""
-    _require(rows > 0 and rot >= 0 and rot % 2 == 0, "rope_table: rows > 0 and an even rot are wanted")
+    if rows <= 0 or rot < 0 or rot % 2:
+        raise ValueError(f"rope_table: rows > 0 and an even rot are wanted, got {rows}, {rot}")
     angle = np.arange(rows, dtype=np.float64)[:, None] * float(base) ** (-np.arange(0, rot, 2, dtype=np.float64) / max(rot, 1))
     return tuple(torch.from_numpy(f(angle).astype(np.float32)).to(device) for f in (np.cos, np.sin))
 
 
 def _heads(t, like, name):
-    """[B, L, h, d] with contiguous d and any other strides; None for no heads."""
-    if t is None:
-        _require(like is None, f"{name} is missing")
+    """The view of `t`, which has the shape, type and device of `like` [B, L, h, d], contiguous d and any other strides; None for no
+    heads."""
+    if t is None or like is None:
+        if t is not like:
+            raise ValueError(f"{name}: missing, or without its input")
         return None
-    _require(like is not None, f"{name} without its input")
-    _require(t.shape == like.shape and t.dtype == like.dtype and t.device == like.device, f"{name}: shape, type and device of its input are wanted")
-    _require(t.shape[3] == 1 or t.stride(3) == 1, f"{name}: the head dim must be contiguous")
-    return C.byref(Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)))
+    sb, sl, sh, sd = t.stride() if t.dim() == 4 else (0, 0, 0, 0)
+    if t is not like and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device) or (sd != 1 and t.shape[-1] != 1):
+        _refuse(name, t, f"{tuple(like.shape)} of {like.dtype} on {like.device} with a contiguous head dim")
+    return Heads(t.data_ptr(), sb, sl, sh)
 
 
 def _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved):
     t = Q if Q is not None else K
-    _require(t is not None and t.dim() == 4 and t.is_cuda and t.dtype in TYPE, "Q, K: [B, L, heads, d] of fp32, fp16 or bf16 on the GPU are wanted")
-    _require(norm in NORM, f"norm: one of {sorted(NORM)}")
-    B, L, _, d = t.shape
-    if Q is not None and K is not None:
-        _require(K.dim() == 4 and K.shape[:2] == Q.shape[:2] and K.shape[3] == d and K.dtype == Q.dtype and K.device == Q.device,
-                 "Q and K: the same batch, length, head dim, type and device are wanted")
-    rows = rot = 0
-    _require((cos is None) == (sin is None), "cos and sin come together")
-    if cos is not None:
-        _require(cos.dim() == 2 and cos.shape == sin.shape, "cos, sin: [rows, rot / 2] are wanted")
-        rows, rot = cos.shape[0], 2 * cos.shape[1]
-        for x in (cos, sin):
-            _require(x.device == t.device and x.dtype == torch.float32 and x.is_contiguous(), f"cos, sin: contiguous fp32 on {t.device} are wanted")
-    pos_b = 0
+    if t is None or t.dim() != 4 or not t.is_cuda or t.dtype not in TYPE:
+        raise ValueError("Q, K: [B, L, heads, d] of fp32, fp16 or bf16 on the GPU are wanted")
+    if norm not in NORM:
+        raise ValueError(f"norm: one of {sorted(NORM)}")
+    B, L, hq, d = t.shape
+    hk, dev = 0, t.device
+    if Q is None:
+        hq, hk = 0, hq
+    elif K is not None:
+        if K.dim() != 4 or K.dtype != t.dtype or K.device != dev or K.shape[0] != B or K.shape[1] != L or K.shape[3] != d:
+            _refuse("K", K, f"[{B}, {L}, heads, {d}] of {t.dtype} on {dev}")
+        hk = K.shape[2]
+    rows = rot = pos_b = 0
+    c = s = p = None
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 or \
+                cos.device != dev or sin.device != dev or not cos.is_contiguous() or not sin.is_contiguous():
+            raise ValueError(f"cos and sin: [rows, rot / 2], contiguous fp32 on {dev}, are wanted")
+        rows, rot = cos.shape
+        rot *= 2
+        if rot:
+            c, s = cos.data_ptr(), sin.data_ptr()
     if positions is not None:
-        _require(positions.device == t.device and positions.dtype == torch.int32, f"positions: int32 on {t.device} are wanted")
-        _require(tuple(positions.shape) in ((L,), (B, L)) and (L <= 1 or positions.stride(-1) == 1), "positions: [L] or [B, L] with contiguous rows are wanted")
-        pos_b = positions.stride(0) if positions.dim() == 2 else 0
-    cfg = QkCfg(B, L, 0 if Q is None else Q.shape[2], 0 if K is None else K.shape[2], d, TYPE[t.dtype], NORM[norm], float(eps), rot,
-                int(bool(interleaved)), rows, pos_b)
-    weights = (_vector(q_weight, d, t.device, "q_weight"), _vector(k_weight, d, t.device, "k_weight"))
-    table = (_p(cos), _p(sin)) if rot else (None, None)
-    return t, cfg, (_heads(Q, Q, "Q"), _heads(K, K, "K"), *weights, *table, _p(positions))
+        shape = positions.shape
+        if positions.device != dev or positions.dtype != torch.int32 or shape[-1] != L or (L > 1 and positions.stride(-1) != 1) or \
+                not (len(shape) == 1 or len(shape) == 2 and shape[0] == B):
+            _refuse("positions", positions, f"[{L}] or [{B}, {L}] int32 on {dev} with contiguous rows")
+        pos_b, p = positions.stride(0) if len(shape) == 2 else 0, positions.data_ptr()
+    cfg = QkCfg(B, L, hq, hk, d, TYPE[t.dtype], NORM[norm], eps, rot, 1 if interleaved else 0, rows, pos_b)
+    return dev, cfg, (cfg, _heads(Q, Q, "Q"), _heads(K, K, "K"), _vec(q_weight, d, dev, "q_weight"), _vec(k_weight, d, dev, "k_weight"), c, s, p)
 
 
 def qk_norm_rope(Q, K, q_weight=None, k_weight=None, norm="rms", eps=1e-6, cos=None, sin=None, positions=None, interleaved=False, out=None):
@@ -322,12 +374,16 @@ def qk_norm_rope(Q, K, q_weight=None, k_weight=None, norm="rms", eps=1e-6, cos=N
     2 * cos.shape[1] dims by row `positions` (int32 [B, L] or [L]; None: 0, 1, ...) of cos / sin (rope_table).  A token with a
     negative position is padding and left alone.  Returns (Q', K'): `out` (tensors of the inputs' shapes and types, any strides; the
     inputs themselves for a pass in place), or new [B, L, h, d] tensors."""
-    t, cfg, args = _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved)
-    with torch.cuda.device(t.device):
-        if out is None:
-            out = tuple(None if x is None else torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (Q, K))
-        rc = _lib.load().ppml_b200_qk_norm_rope(C.byref(cfg), *args, _heads(out[0], Q, "out[0]"), _heads(out[1], K, "out[1]"), _stream())
-    _check(rc, "qk_norm_rope")
+    dev, _, args = _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved)
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return qk_norm_rope(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved, out)
+    if out is None:
+        out = tuple(None if x is None else torch.empty(x.shape, device=dev, dtype=x.dtype) for x in (Q, K))
+    rc = _lib.load().ppml_b200_qk_norm_rope(*args, _heads(out[0], Q, "out[0]"), _heads(out[1], K, "out[1]"), _raw_stream(dev))
+    if rc:
+        _check(rc, "qk_norm_rope")
     return out
 
 
@@ -335,21 +391,28 @@ def qk_norm_rope_backward(Q, K, dQo, dKo, q_weight=None, k_weight=None, norm="rm
                           interleaved=False, out=None):
     """Gradients of qk_norm_rope from its inputs Q, K and the gradients dQo, dKo of its results (their shapes, any strides).  Returns
     a dict: dQ, dK (`out`: tensors to write them into) and, for the weights that are given, dq_weight, dk_weight [d] fp32."""
-    t, cfg, args = _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved)
+    dev, cfg, args = _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved)
+    guard = _on(dev)
+    if guard is not None:
+        with guard:
+            return qk_norm_rope_backward(Q, K, dQo, dKo, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved, out)
     lib = _lib.load()
-    with torch.cuda.device(t.device):
-        if out is None:
-            out = tuple(None if x is None else torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (Q, K))
-        got = {"dQ": out[0], "dK": out[1]}
-        for name, w in (("dq_weight", q_weight), ("dk_weight", k_weight)):
+    if out is None:
+        out = tuple(None if x is None else torch.empty(x.shape, device=dev, dtype=x.dtype) for x in (Q, K))
+    got = {n: x for n, x in (("dQ", out[0]), ("dK", out[1])) if x is not None}
+    dw, ws, need = [None, None], None, 0
+    if q_weight is not None or k_weight is not None:
+        for i, (n, w) in enumerate((("dq_weight", q_weight), ("dk_weight", k_weight))):
             if w is not None:
-                got[name] = torch.empty_like(w)
-        need = lib.ppml_b200_qk_norm_rope_backward_workspace(C.byref(cfg)) if len(got) > 2 else 0
-        ws = torch.empty(need, device=t.device, dtype=torch.uint8) if need else None
-        rc = lib.ppml_b200_qk_norm_rope_backward(C.byref(cfg), *args, _heads(dQo, Q, "dQo"), _heads(dKo, K, "dKo"), _heads(out[0], Q, "dQ"),
-                                                 _heads(out[1], K, "dK"), _p(got.get("dq_weight")), _p(got.get("dk_weight")), _p(ws), need, _stream())
-    _check(rc, "qk_norm_rope_backward")
-    return {n: v for n, v in got.items() if v is not None}
+                got[n] = torch.empty(w.shape, device=dev, dtype=torch.float32)
+                dw[i] = got[n].data_ptr()
+        need = lib.ppml_b200_qk_norm_rope_backward_workspace(cfg)
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+    rc = lib.ppml_b200_qk_norm_rope_backward(*args, _heads(dQo, Q, "dQo"), _heads(dKo, K, "dKo"), _heads(out[0], Q, "dQ"), _heads(out[1], K, "dK"),
+                                             *dw, None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
+    if rc:
+        _check(rc, "qk_norm_rope_backward")
+    return got
 
 
 def flash_attn_forward_cuda(Q, K, V, bias=None, scale=0.0, causal=False, eps=1e-9, bias_bcast=False, path=PATH_AUTO, out=None,
