@@ -303,7 +303,10 @@ int check_i8(const int8_t* B, int64_t ldb, const float* b_scale, const void* C, 
     return ST_OK;
 }
 int i8_product(const I8Product& p, int path, cudaStream_t st) {
-    if (path == PPML_B200_PATH_UMMA) return ST_UNSUPPORTED_PATH;
+    if (path != PPML_B200_PATH_SIMT) {
+        const int rc = launch_umma_i8(p, st);
+        if (rc != ST_UNSUPPORTED_PATH || path == PPML_B200_PATH_UMMA) return rc;
+    }
     return launch_i8_dp4a(p, st);
 }
 }  // namespace

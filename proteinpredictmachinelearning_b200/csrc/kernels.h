@@ -134,6 +134,8 @@ struct I8Product {
 int launch_quantize_tokens(const void* x, int type, long long ld_x, int8_t* q, long long ld_q, float* scale, long long rows, int K,
                            cudaStream_t st);
 int launch_i8_dp4a(const I8Product& p, cudaStream_t st);
+// tcgen05 (umma_i8.cu): 16-byte aligned operands and pitches, ST_UNSUPPORTED_PATH otherwise
+int launch_umma_i8(const I8Product& p, cudaStream_t st);
 
 // Per-head norms of Q and K with the position rotation (qk_norm_rope.cu).  Element (b, l, h, i) of a view is at
 // p[b * b_stride + l * l_stride + h * h_stride + i].

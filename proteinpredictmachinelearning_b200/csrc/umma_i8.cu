@@ -1,0 +1,481 @@
+// umma_i8.cu -- C[token][channel] = epilogue(sum_k A[token][k] * W[channel][k]) in 8-bit integers on tcgen05 (kind::i8).
+//
+// The weights are the tensor core's M operand and the tokens its N operand: the accumulator then holds a channel per TMEM lane
+// and a token per column, a warp that reads one column holds 32 neighbouring channels of one token, and the results leave the
+// registers as whole coalesced pieces of a row of C, whatever its pitch and type.  The whole sum over K stays in int32 in
+// TMEM, so splitting K changes nothing; each output sees one epilogue.
+//
+// Both operands are K-major int8 tiles of 128 bytes of K per stage (128-byte swizzle), pulled in by TMA; rows and K beyond the
+// tensors read as zeros.  Warp 0 = TMA, warp 1 = MMA issue and TMEM owner, warps 2 - 9 = epilogue (two per TMEM lane quarter).
+#include "i8_common.cuh"
+#include "tma_host.h"
+
+namespace ppml_b200 {
+namespace {
+
+constexpr int kThreadsI8 = 320;
+constexpr int kFirstEpi = 2, kEpiWarps = 8;
+constexpr int kMaxStages = 8;
+constexpr int kRowsA = 128;                        // channels per CTA
+constexpr int kABytes = kRowsA * 128;
+constexpr int kBarBytes = 256, kScaleBytes = kEpiWarps * 32 * 4;
+
+struct I8Tc {
+    I8Product p;
+    int bn;                                        // tokens per tile (the MMA's N): a multiple of 16 (pairs: of 32), at most 256
+    int stages, stage_bytes;
+    int tiles_n, tiles_t, kblocks;
+    int tmem_cols;                                 // power of two >= what the accumulators take
+    int* err;
+};
+
+// ---- cluster helpers ----
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t map_to(uint32_t saddr, uint32_t rank) {
+    uint32_t r; asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank)); return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ int ld_cluster_s32(uint32_t cluster_addr) {
+    int v; asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory"); return v;
+}
+
+// ---- the forms that a pair of CTAs uses ----
+template <int CG> __device__ __forceinline__ void tmem_alloc_cg(uint32_t dst, uint32_t n) {
+    if constexpr (CG == 1) tmem_alloc(dst, n);
+    else asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(n) : "memory");
+}
+template <int CG> __device__ __forceinline__ void tmem_free_cg(uint32_t taddr, uint32_t n) {
+    if constexpr (CG == 1) { tmem_relinquish(); tmem_dealloc(taddr, n); }
+    else {
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(n) : "memory");
+    }
+}
+// CG = 2: into this CTA's shared memory, counted on a barrier of the pair's leader
+template <int CG> __device__ __forceinline__ void load_tile(uint32_t dst, const void* tm, uint32_t bar, int x, int y) {
+    if constexpr (CG == 1) tma_load_3d(dst, tm, bar, x, y, 0);
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];"
+            ::"r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(x), "r"(y), "r"(0) : "memory");
+}
+template <int CG> __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    if constexpr (CG == 1) umma<MmaKind::I8>(d, a, b, idesc, acc);
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// arrives on the barrier at this offset in every CTA of the group once all MMAs issued so far are done
+template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (CG == 1) umma_commit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+
+// ---- epilogue of 32 tokens x this lane's channel ----
+template <typename T>
+__device__ __forceinline__ void store_chunk(const I8Product& p, const int (&sum)[32], float* scale_buf, long long t0, int left, long long n,
+                                            bool n_ok, float b_scale, float bias, int lane) {
+    // left = tokens of the chunk that exist (may be <= 0)
+    __syncwarp();
+    scale_buf[lane] = lane < left ? p.a_scale[t0 + lane] : 0.0f;
+    __syncwarp();
+    if (!n_ok) return;
+    T* c = static_cast<T*>(p.C) + t0 * p.ldc + n;
+    const T* g = static_cast<const T*>(p.gate) + t0 * p.ld_gate + n;
+#pragma unroll
+    for (int j0 = 0; j0 < 32; j0 += 8) {
+        float y[8];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const float4 s = reinterpret_cast<const float4*>(scale_buf)[j0 / 4 + q];
+            y[4 * q] = fmaf(static_cast<float>(sum[j0 + 4 * q]) * s.x, b_scale, bias);
+            y[4 * q + 1] = fmaf(static_cast<float>(sum[j0 + 4 * q + 1]) * s.y, b_scale, bias);
+            y[4 * q + 2] = fmaf(static_cast<float>(sum[j0 + 4 * q + 2]) * s.z, b_scale, bias);
+            y[4 * q + 3] = fmaf(static_cast<float>(sum[j0 + 4 * q + 3]) * s.w, b_scale, bias);
+        }
+        if (p.act != 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = i8_act(p.act, y[j]);
+        }
+        if (p.gate) {
+            float gv[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) gv[j] = j0 + j < left ? to_f32(g[(j0 + j) * p.ld_gate]) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= gv[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < left) c[(j0 + j) * p.ldc] = from_f32<T>(y[j]);
+    }
+}
+
+// On an abort the copies that are still on their way must not land in the shared memory of a later block.
+__device__ __noinline__ void wait_for_copies() {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000LL) __nanosleep(1000);
+}
+
+// Persistent: a CTA (CG = 1) or a pair of CTAs (CG = 2: 256 channels, each CTA holding half of the weight rows and half of the
+// token rows of a stage) takes every gridDim-th tile; two accumulators in TMEM, so that a tile's epilogue runs under the
+// next tile's MMAs.
+template <typename T, int CG>
+__global__ void __launch_bounds__(kThreadsI8, 1)
+i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const I8Tc q) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + q.stages * q.stage_bytes;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
+    auto tfull = [&](int a) { return bars + 8u * (2 * kMaxStages + a); };
+    auto tempty = [&](int a) { return bars + 8u * (2 * kMaxStages + 2 + a); };
+    uint8_t* tail = gen + q.stages * q.stage_bytes;
+    volatile int* cta_abort = reinterpret_cast<volatile int*>(tail + 8 * (2 * kMaxStages + 4));
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 8 * (2 * kMaxStages + 4) + 8);
+    float* scales = reinterpret_cast<float*>(tail + kBarBytes);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? cluster_rank() : 0u;
+    const int group = blockIdx.x / CG, groups = gridDim.x / CG;
+    const int tiles = q.tiles_n * q.tiles_t;
+
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&tmW); prefetch_tmap(&tmA);
+        for (int s = 0; s < q.stages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(tfull(a), 1); mbar_init(tempty(a), CG * kEpiWarps); }
+        *cta_abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc_cg<CG>(smem_u32(tmem_slot), q.tmem_cols);
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    // tile index -> (channel tile, token tile): eight token tiles side by side, so that tiles in flight share operands in L2
+    auto tile_at = [&](int i, int& tn, int& tt) {
+        const int per = 8 * q.tiles_n, g = i / per, first = g * 8, r = i - g * per;
+        const int width = min(8, q.tiles_t - first);
+        tn = r / width; tt = first + r - tn * width;
+    };
+    const int b_rows = q.bn / CG;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0; uint32_t ph = 0; bool ok = true;
+            int issued = 0;
+            for (int i = group; i < tiles && ok; i += groups) {
+                int tn, tt; tile_at(i, tn, tt);
+                const int yw = tn * kRowsA * CG + static_cast<int>(rank) * kRowsA;
+                const int ya = tt * q.bn + static_cast<int>(rank) * b_rows;
+                for (int kb = 0; kb < q.kblocks; ++kb) {
+                    if (!mbar_wait(empty(s), ph ^ 1u, cta_abort, q.err, 0x800 | s)) { ok = false; break; }
+                    const uint32_t at = base + s * q.stage_bytes;
+                    const uint32_t bar = CG == 2 ? map_to(full(s), 0) : full(s);
+                    if (rank == 0) mbar_arrive_expect_tx(full(s), static_cast<uint32_t>(CG * q.stage_bytes));
+                    load_tile<CG>(at, &tmW, bar, kb * 128, yw);
+                    load_tile<CG>(at + kABytes, &tmA, bar, kb * 128, ya);
+                    ++issued;
+                    if (++s == q.stages) { s = 0; ph ^= 1u; }
+                }
+            }
+            // every stage has been handed back before this CTA may leave: commits of the pair still arrive here
+            for (int n = min(issued, q.stages); n > 0 && ok; --n) {
+                if (issued < q.stages && n == issued) { s = 0; ph = 1u; }      // fewer loads than stages: the first ones, phase 0
+                ok = mbar_wait(empty(s), ph ^ 1u, cta_abort, q.err, 0x810 | s);
+                if (++s == q.stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = make_idesc(2, 1, 1, 0, 0, kRowsA * CG, q.bn);
+            const int last_steps = (q.p.K - (q.kblocks - 1) * 128 + 31) / 32;
+            int s = 0; uint32_t ph = 0; bool ok = true; int acc = 0; uint32_t aph = 0;
+            for (int i = group; i < tiles && ok; i += groups) {
+                if (!mbar_wait(tempty(acc), aph ^ 1u, cta_abort, q.err, 0x820 | acc)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * (q.tmem_cols / 2);
+                for (int kb = 0; kb < q.kblocks; ++kb) {
+                    if (!mbar_wait(full(s), ph, cta_abort, q.err, 0x830 | s)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at = base + s * q.stage_bytes;
+                    const uint64_t da = make_smem_desc(at, 16, 1024, kLayoutSW128), db = make_smem_desc(at + kABytes, 16, 1024, kLayoutSW128);
+                    const int steps = kb == q.kblocks - 1 ? last_steps : 4;
+                    for (int k = 0; k < steps; ++k) mma_i8<CG>(d, da + 2 * k, db + 2 * k, idesc, kb != 0 || k != 0);
+                    commit<CG>(empty(s));
+                    if (++s == q.stages) { s = 0; ph ^= 1u; }
+                }
+                if (!ok) break;
+                commit<CG>(tfull(acc));
+                if (++acc == 2) { acc = 0; aph ^= 1u; }
+            }
+        }
+    } else {
+        const int quarter = warp & 3, part = (warp - kFirstEpi) >> 2;
+        float* scale_buf = scales + (warp - kFirstEpi) * 32;
+        int acc = 0; uint32_t aph = 0;
+        for (int i = group; i < tiles; i += groups) {
+            int tn, tt; tile_at(i, tn, tt);
+            const long long n = static_cast<long long>(tn) * kRowsA * CG + rank * kRowsA + quarter * 32 + lane;
+            const bool n_ok = n < q.p.N;
+            const float bs = n_ok ? q.p.b_scale[n] : 0.0f, bias = n_ok && q.p.bias ? q.p.bias[n] : 0.0f;
+            const long long t0 = static_cast<long long>(tt) * q.bn;
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull(acc), aph, cta_abort, q.err, 0x840 | acc))) break;
+            tc_fence_after();
+            const uint32_t d = tmem + acc * (q.tmem_cols / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
+            const long long rest = q.p.M - t0;
+            const int cols = static_cast<int>(rest < q.bn ? rest : q.bn);
+            for (int c = part * 32; c < cols; c += 64) {
+                uint32_t r[32];
+                __syncwarp();
+                tmem_ld32(d + c, r);
+                tmem_ld_wait();
+                if (c + 64 >= cols) {              // the last read of this warp: the accumulator may be written again
+                    tc_fence_before();
+                    if (lane == 0) { if (CG == 2) mbar_arrive_cluster(map_to(tempty(acc), 0)); else mbar_arrive(tempty(acc)); }
+                }
+                int v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = static_cast<int>(r[j]);
+                store_chunk<T>(q.p, v, scale_buf, t0 + c, min(32, cols - c), n, n_ok, bs, bias, lane);
+            }
+            if (part * 32 >= cols && lane == 0) {  // nothing to read in this tile
+                if (CG == 2) mbar_arrive_cluster(map_to(tempty(acc), 0)); else mbar_arrive(tempty(acc));
+            }
+            if (++acc == 2) { acc = 0; aph ^= 1u; }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*cta_abort && threadIdx.x == 0) wait_for_copies();
+    __syncwarp();
+    if (CG == 2) cluster_sync_all();
+    tc_fence_after();
+    if (warp == 1) tmem_free_cg<CG>(tmem, q.tmem_cols);
+}
+
+// Few tiles: one tile per cluster of `parts` CTAs, each of which sums its share of K; the int32 partial sums meet in shared
+// memory, every CTA finishing its share of the tokens.
+template <typename T>
+__global__ void __launch_bounds__(kThreadsI8, 1)
+i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const I8Tc q, const int parts) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    const uint32_t bars = base + q.stages * q.stage_bytes;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
+    const uint32_t tfull = bars + 8u * 2 * kMaxStages;
+    uint8_t* tail = gen + q.stages * q.stage_bytes;
+    volatile int* cta_abort = reinterpret_cast<volatile int*>(tail + 8 * (2 * kMaxStages + 4));
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tail + 8 * (2 * kMaxStages + 4) + 8);
+    float* scales = reinterpret_cast<float*>(tail + kBarBytes);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = parts > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int tile = blockIdx.x / parts, tn = tile / q.tiles_t, tt = tile - tn * q.tiles_t;
+    const int kb0 = static_cast<int>(static_cast<long long>(q.kblocks) * rank / parts);
+    const int kb1 = static_cast<int>(static_cast<long long>(q.kblocks) * (rank + 1) / parts);
+
+    if (threadIdx.x == 0) {
+        prefetch_tmap(&tmW); prefetch_tmap(&tmA);
+        for (int s = 0; s < q.stages; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        mbar_init(tfull, 1);
+        *cta_abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), q.tmem_cols);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait();
+    pdl_launch_dependents();
+
+    const long long t0 = static_cast<long long>(tt) * q.bn;
+    const long long rest = q.p.M - t0;
+    const int cols = static_cast<int>(rest < q.bn ? rest : q.bn);
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0; uint32_t ph = 0;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(empty(s), ph ^ 1u, cta_abort, q.err, 0x900 | s)) break;
+                const uint32_t at = base + s * q.stage_bytes;
+                mbar_arrive_expect_tx(full(s), static_cast<uint32_t>(q.stage_bytes));
+                load_tile<1>(at, &tmW, full(s), kb * 128, tn * kRowsA);
+                load_tile<1>(at + kABytes, &tmA, full(s), kb * 128, static_cast<int>(t0));
+                if (++s == q.stages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = make_idesc(2, 1, 1, 0, 0, kRowsA, q.bn);
+            const int last_steps = (q.p.K - (q.kblocks - 1) * 128 + 31) / 32;
+            int s = 0; uint32_t ph = 0; bool ok = true;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait(full(s), ph, cta_abort, q.err, 0x930 | s)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t at = base + s * q.stage_bytes;
+                const uint64_t da = make_smem_desc(at, 16, 1024, kLayoutSW128), db = make_smem_desc(at + kABytes, 16, 1024, kLayoutSW128);
+                const int steps = kb == q.kblocks - 1 ? last_steps : 4;
+                for (int k = 0; k < steps; ++k) umma<MmaKind::I8>(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
+                umma_commit(empty(s));
+                if (++s == q.stages) { s = 0; ph ^= 1u; }
+            }
+            if (ok) umma_commit(tfull);
+        }
+    }
+    __syncwarp();
+    const int quarter = warp & 3, part = (warp - kFirstEpi) >> 2;
+    const long long n = static_cast<long long>(tn) * kRowsA + quarter * 32 + lane;
+    const bool n_ok = n < q.p.N;
+    const float bs = n_ok ? q.p.b_scale[n] : 0.0f, bias = n_ok && q.p.bias ? q.p.bias[n] : 0.0f;
+    float* scale_buf = scales + (warp - kFirstEpi) * 32;
+    if (warp >= kFirstEpi) {
+        if (__all_sync(0xffffffffu, mbar_wait(tfull, 0, cta_abort, q.err, 0x940))) {
+            tc_fence_after();
+            for (int c = part * 32; c < cols; c += 64) {
+                uint32_t r[32];
+                __syncwarp();
+                tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
+                tmem_ld_wait();
+                int v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = static_cast<int>(r[j]);
+                if (parts == 1) {
+                    store_chunk<T>(q.p, v, scale_buf, t0 + c, min(32, cols - c), n, n_ok, bs, bias, lane);
+                } else {                           // the stages are free: every load has landed and every MMA has read
+                    int* buf = reinterpret_cast<int*>(gen) + c * kRowsA + quarter * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) buf[j * kRowsA] = v[j];
+                }
+            }
+        }
+    }
+    if (parts > 1) {
+        __syncwarp();
+        cluster_sync_all();
+        if (warp >= kFirstEpi) {
+            // tokens in chunks of 8, chunk u to the CTA u mod parts, alternating between the two halves of the warps
+            int turn = 0;
+            for (int c = rank * 8; c < cols; c += 8 * parts, turn ^= 1) {
+                if (turn != part) continue;
+                int v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0;
+                const uint32_t at = base + static_cast<uint32_t>((c * kRowsA + quarter * 32 + lane) * 4);
+                for (int r = 0; r < parts; ++r) {
+                    const uint32_t there = map_to(at, static_cast<uint32_t>((rank + r) % parts));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += ld_cluster_s32(there + j * kRowsA * 4);
+                }
+                store_chunk<T>(q.p, v, scale_buf, t0 + c, min(8, cols - c), n, n_ok, bs, bias, lane);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (*cta_abort && threadIdx.x == 0) wait_for_copies();
+    __syncwarp();
+    if (parts > 1) cluster_sync_all();
+    tc_fence_after();
+    if (warp == 1) { tmem_relinquish(); tmem_dealloc(tmem, q.tmem_cols); }
+}
+
+int pow2_at_least(int v, int lo) { int c = lo; while (c < v) c *= 2; return c; }
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), int grid, int cluster, size_t smem, cudaStream_t st, Args... args) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kThreadsI8); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+struct Plan { int pair, bn, parts; };              // pair: 0 parts kernel, 1 persistent single CTAs, 2 persistent pairs
+
+Plan choose(const I8Product& p) {
+    const long long sms = num_sms();
+    const int kblocks = (p.K + 127) / 128;
+    const long long tn = (p.N + 127) / 128;
+    auto tt = [&](int bn) { return (p.M + static_cast<long long>(bn) - 1) / bn; };
+    Plan plan{0, 0, 1};
+    const int cap = p.M >= 128 ? 128 : (p.M + 15) / 16 * 16;
+    if (tn * tt(128) > sms) {
+        plan.pair = p.N > 128 ? 2 : 1;
+        plan.bn = 256;
+        while (plan.bn > 64 && (tn + plan.pair - 1) / plan.pair * tt(plan.bn) * plan.pair < 4 * sms && kblocks <= 8) plan.bn /= 2;
+        return plan;
+    }
+    plan.bn = cap;
+    while (plan.bn > 32 && tn * tt(plan.bn) * 2 <= sms && kblocks < 8) plan.bn = (plan.bn / 2 + 15) / 16 * 16;
+    const long long tiles = tn * tt(plan.bn);
+    while (plan.parts < 8 && tiles * plan.parts * 2 <= sms && kblocks >= 4 * plan.parts) plan.parts *= 2;
+    return plan;
+}
+
+template <typename T>
+int launch_t(const I8Product& p, const Plan& plan, cudaStream_t st) {
+    const int cg = plan.pair == 2 ? 2 : 1;
+    I8Tc q{};
+    q.p = p; q.bn = plan.bn;
+    q.stage_bytes = kABytes + plan.bn / cg * 128;
+    q.stages = 200 * 1024 / q.stage_bytes;
+    if (q.stages > kMaxStages) q.stages = kMaxStages;
+    q.kblocks = (p.K + 127) / 128;
+    q.tiles_n = static_cast<int>((p.N + static_cast<long long>(kRowsA) * cg - 1) / (kRowsA * cg));
+    q.tiles_t = static_cast<int>((p.M + static_cast<long long>(plan.bn) - 1) / plan.bn);
+    if (static_cast<long long>(q.tiles_n) * q.tiles_t > INT32_MAX / 8) return ST_UNSUPPORTED_PATH;
+    q.err = device_error_ptr();
+    if (!q.err) return ST_LAUNCH;
+    CUtensorMap tmW, tmA;
+    if (!make_tmap_3d(&tmW, TmaType::U8, p.B, p.K, p.N, 1, p.ldb, 0, 128, kRowsA, 1) ||
+        !make_tmap_3d(&tmA, TmaType::U8, p.A, p.K, p.M, 1, p.lda, 0, 128, plan.bn / cg, 1))
+        return ST_UNSUPPORTED_PATH;
+    const size_t smem = static_cast<size_t>(q.stages) * q.stage_bytes + kBarBytes + kScaleBytes + 1024;
+    cudaError_t e;
+    if (plan.pair == 0) {
+        q.tmem_cols = pow2_at_least(plan.bn, 32);
+        e = launch_cluster(i8_parts_kernel<T>, q.tiles_n * q.tiles_t * plan.parts, plan.parts, smem, st, tmW, tmA, q, plan.parts);
+    } else {
+        q.tmem_cols = 2 * pow2_at_least(plan.bn, 32);
+        const int units = q.tiles_n * q.tiles_t, most = num_sms() / cg, groups = units < most ? units : most;
+        e = cg == 2 ? launch_cluster(i8_tiles_kernel<T, 2>, groups * 2, 2, smem, st, tmW, tmA, q)
+                    : launch_cluster(i8_tiles_kernel<T, 1>, groups, 1, smem, st, tmW, tmA, q);
+    }
+    if (e != cudaSuccess) { cudaGetLastError(); return ST_LAUNCH; }
+    return ST_OK;
+}
+
+}  // namespace
+
+int launch_umma_i8(const I8Product& p, cudaStream_t st) {
+    if ((reinterpret_cast<uintptr_t>(p.A) | reinterpret_cast<uintptr_t>(p.B) | p.lda | p.ldb) & 15) return ST_UNSUPPORTED_PATH;
+    const Plan plan = choose(p);
+    return p.c_type == kTypeF32 ? launch_t<float>(p, plan, st)
+                                : p.c_type == kTypeF16 ? launch_t<__half>(p, plan, st) : launch_t<__nv_bfloat16>(p, plan, st);
+}
+
+}  // namespace ppml_b200

@@ -153,6 +153,20 @@ def test_product_against_64_bits(M, K, N, path, no_device_abort):
 
 
 @gpu
+@pytest.mark.parametrize("M,K,N", [(19001, 144, 96), (40003, 48, 120), (5001, 272, 600), (2600, 1104, 1100), (9000, 2064, 264), (65536, 32, 136),
+                                   (1111, 4100, 2056), (300, 128, 20011)])
+def test_many_tiles(M, K, N, no_device_abort):
+    """More output tiles than SMs, with one and two tiles of channels, one to many steps of K, ragged ends on every side."""
+    A, W, sa, sw, bias = ints(M, K, 1), ints(N, K, 2), scales(M, 3), scales(N, 4), scales(N, 5)
+    gate = torch.randn((M, N), generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    out = torch.full((M + 1, N + 3), -7.0, device="cuda")
+    ops.mul_mat_i8(A, sa, W, sw, bias=bias, gate=gate, out=out[:M, :N])
+    check_product(out[:M, :N], A, sa, W, sw, bias, gate, "none")
+    assert (out[:, N:] == -7).all() and (out[M] == -7).all()
+    check_product(ops.mul_mat_i8(A, sa, W, sw, act="silu", dtype=BF16), A, sa, W, sw, None, None, "silu")
+
+
+@gpu
 @pytest.mark.parametrize("M,K,N", [(1, 1024, 256), (5, 80, 40), (24, 512, 264), (140, 64, 96), (300, 256, 520), (33, 100, 41)])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("act", ["none", "sigmoid", "silu", "gelu", "tanh", "relu"])
