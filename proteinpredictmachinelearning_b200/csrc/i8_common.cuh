@@ -37,6 +37,66 @@ __device__ __forceinline__ int i8_quantize(float x, float scale) {
     const float r = rintf(__fdiv_rn(x, scale));
     return static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
 }
+// 1 / scale for i8_quantize4; 0 where its shortcut does not hold
+__device__ __forceinline__ float i8_inverse(float scale) { return scale > 1e-30f && scale < 1e30f ? __frcp_rn(scale) : 0.0f; }
+// Four values as packed bytes, the same as i8_quantize.  x * (1 / scale) is within 127 * 2^-23 of the rounded quotient, so the two
+// round alike unless the product lies within 2^-14 of a half: only then is the quotient itself taken.  Adding 1.5 * 2^23 rounds
+// to an integer (half to even) whose low byte is the result.
+__device__ __forceinline__ uint32_t i8_quantize4(const float (&x)[4], float scale, float inv) {
+    constexpr float kRound = 12582912.0f;
+    float t[4], off = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = x[i] * inv;
+        t[i] = y + kRound;
+        off = fmaxf(off, fabsf(y - (t[i] - kRound)));
+    }
+    if (off > 0.5f - 6.103515625e-5f || inv == 0.0f) {
+        uint32_t v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v |= (static_cast<uint32_t>(i8_quantize(x[i], scale)) & 255u) << (8 * i);
+        return v;
+    }
+    const uint32_t lo = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+}
+
+// 16 bytes of a row of x
+template <typename T> struct Vec16 { static constexpr int kN = 16 / sizeof(T); };
+// the largest magnitude among them, as fp32 bits; 16-bit types are compared two at a time
+template <typename T> __device__ __forceinline__ uint32_t top_of(const uint4& v) {
+    if constexpr (sizeof(T) == 4) {
+        return max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+    } else {
+        const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+        const uint16_t h = static_cast<uint16_t>(max(m & 0xffffu, m >> 16));
+        return magnitude_bits(to_f32(*reinterpret_cast<const T*>(&h)));
+    }
+}
+template <typename T> __device__ __forceinline__ void unpack_vec(const uint4& v, float (&x)[Vec16<T>::kN]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __uint_as_float(w[i]);
+        } else {
+            const uint16_t lo = static_cast<uint16_t>(w[i] & 0xffffu), hi = static_cast<uint16_t>(w[i] >> 16);
+            x[2 * i] = to_f32(*reinterpret_cast<const T*>(&lo));
+            x[2 * i + 1] = to_f32(*reinterpret_cast<const T*>(&hi));
+        }
+    }
+}
+// 16 bytes of x as 4 (fp32) or 8 integers
+template <typename T> __device__ __forceinline__ void quantize_vec(const uint4& v, float scale, float inv, uint32_t (&q)[Vec16<T>::kN / 4]) {
+    float x[Vec16<T>::kN];
+    unpack_vec<T>(v, x);
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::kN / 4; ++i) {
+        const float f[4] = {x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+        q[i] = i8_quantize4(f, scale, inv);
+    }
+}
 
 // The activations of act_scalar with sigmoid, SiLU and GELU through the hardware's exp2 and reciprocal (about 2 ulp each, the
 // exponent's argument rounded once; expf and an IEEE division cost a dozen instructions more per output):
@@ -56,6 +116,13 @@ __device__ __forceinline__ float i8_act(int kind, float x) {
         case 5: return x < 0.0f ? 0.0f : x;            // keeps NaN
         default: return x;
     }
+}
+// the same for N values: one branch on the kind
+template <int N>
+__device__ __forceinline__ void i8_act_all(int kind, float (&y)[N]) {
+#define PPML_ACT(K) case K: { _Pragma("unroll") for (int j = 0; j < N; ++j) y[j] = i8_act(K, y[j]); break; }
+    switch (kind) { PPML_ACT(1) PPML_ACT(2) PPML_ACT(3) PPML_ACT(4) PPML_ACT(5) default: break; }
+#undef PPML_ACT
 }
 __device__ __forceinline__ float i8_epilogue(int sum, float a_scale, float b_scale, float bias, int act) {
     return i8_act(act, fmaf(static_cast<float>(sum) * a_scale, b_scale, bias));

@@ -5,22 +5,93 @@
 namespace ppml_b200 {
 namespace {
 
-// One block per row; the second pass over the row comes from L1 / L2.
+// ---- quantizer: one pass over x ----
+// A row per warp (THREADS = 32, eight rows per block) or per block of 256 threads; its NV 16-byte pieces per thread are all
+// requested at once and stay in registers from the maximum to the quotients.  Bound by bandwidth: e + 1 bytes a value.
+template <typename T, int THREADS, int NV>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long long ld_x, int8_t* __restrict__ q, long long ld_q,
+                                                            float* __restrict__ scale, long long M, int K) {
+    constexpr int N = Vec16<T>::kN;
+    __shared__ __align__(16) uint32_t part[8];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5;
+    const long long row = THREADS == 32 ? static_cast<long long>(blockIdx.x) * 8 + warp : blockIdx.x;
+    if (THREADS == 32 && row >= M) return;
+    const int me = THREADS == 32 ? threadIdx.x & 31 : threadIdx.x;
+    const T* xr = x + row * ld_x;
+    uint4 v[NV];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int k = (me + i * THREADS) * N;
+        v[i] = k < K ? *reinterpret_cast<const uint4*>(xr + k) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) top = max(top, top_of<T>(v[i]));
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (THREADS > 32) {
+        if ((threadIdx.x & 31) == 0) part[warp] = top;
+        __syncthreads();
+        const uint4 a = reinterpret_cast<const uint4*>(part)[0], b = reinterpret_cast<const uint4*>(part)[1];
+        top = max(max(max(a.x, a.y), max(a.z, a.w)), max(max(b.x, b.y), max(b.z, b.w)));
+    }
+    const float s = i8_scale(top), inv = i8_inverse(s);
+    int8_t* qr = q + row * ld_q;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int k = (me + i * THREADS) * N;
+        if (k >= K) continue;
+        uint32_t w[N / 4];
+        quantize_vec<T>(v[i], s, inv, w);
+        if constexpr (N == 4) *reinterpret_cast<uint32_t*>(qr + k) = w[0];
+        else *reinterpret_cast<uint2*>(qr + k) = make_uint2(w[0], w[1]);
+    }
+    if (me == 0) scale[row] = s;
+}
+
+// Any length, any alignment: one block per row, value by value; the second pass over the row comes from L1 / L2.
 template <typename T>
-__global__ void __launch_bounds__(128) quantize_tokens_kernel(const T* __restrict__ x, long long ld_x, int8_t* __restrict__ q, long long ld_q,
-                                                              float* __restrict__ scale, int K) {
-    __shared__ uint32_t part[4];
+__global__ void __launch_bounds__(512) quantize_any_kernel(const T* __restrict__ x, long long ld_x, int8_t* __restrict__ q, long long ld_q,
+                                                           float* __restrict__ scale, int K) {
+    __shared__ uint32_t part[16];
+    pdl_wait();
+    pdl_launch_dependents();
     const long long row = blockIdx.x;
     const T* xr = x + row * ld_x;
     uint32_t top = 0;
-    for (int k = threadIdx.x; k < K; k += 128) top = max(top, magnitude_bits(to_f32(xr[k])));
+#pragma unroll 4
+    for (int k = threadIdx.x; k < K; k += blockDim.x) top = max(top, magnitude_bits(to_f32(xr[k])));
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
     __syncthreads();
-    const float s = i8_scale(max(max(part[0], part[1]), max(part[2], part[3])));
+    const int lane = threadIdx.x & 31;
+    const float s = i8_scale(__reduce_max_sync(0xffffffffu, lane < static_cast<int>(blockDim.x >> 5) ? part[lane] : 0u));
     int8_t* qr = q + row * ld_q;
-    for (int k = threadIdx.x; k < K; k += 128) qr[k] = static_cast<int8_t>(i8_quantize(to_f32(xr[k]), s));
+#pragma unroll 4
+    for (int k = threadIdx.x; k < K; k += blockDim.x) qr[k] = static_cast<int8_t>(i8_quantize(to_f32(xr[k]), s));
     if (threadIdx.x == 0) scale[row] = s;
+}
+
+template <typename T>
+int launch_quantize_t(const T* x, long long ld_x, int8_t* q, long long ld_q, float* scale, long long rows, int K, cudaStream_t st) {
+    constexpr int N = Vec16<T>::kN;
+    const bool vec = (reinterpret_cast<uintptr_t>(x) | (ld_x * sizeof(T))) % 16 == 0 && (reinterpret_cast<uintptr_t>(q) | ld_q) % N == 0 && K % N == 0;
+    const int pieces = (K + N - 1) / N;
+    const unsigned by_warp = static_cast<unsigned>((rows + 7) / 8), by_block = static_cast<unsigned>(rows);
+    cudaError_t e;
+#define PPML_Q(THREADS, NV) launch_pdl(quantize_rows_kernel<T, THREADS, NV>, dim3(THREADS == 32 ? by_warp : by_block), dim3(256), 0, st, x, ld_x, q, ld_q, scale, rows, K)
+    if (!vec || pieces > 2048) e = launch_pdl(quantize_any_kernel<T>, dim3(by_block), dim3(K <= 1024 ? 128 : 512), 0, st, x, ld_x, q, ld_q, scale, K);
+    else if (pieces <= 32) e = PPML_Q(32, 1);
+    else if (pieces <= 64) e = PPML_Q(32, 2);
+    else if (pieces <= 128) e = PPML_Q(32, 4);
+    else if (pieces <= 256) e = PPML_Q(256, 1);
+    else if (pieces <= 512) e = PPML_Q(256, 2);
+    else if (pieces <= 1024) e = PPML_Q(256, 4);
+    else e = PPML_Q(256, 8);
+#undef PPML_Q
+    if (e != cudaSuccess) { cudaGetLastError(); return ST_LAUNCH; }
+    return ST_OK;
 }
 
 // 64 x 64 outputs per block of 256 threads, 4 x 4 each; 64 k per step as 16 words of four, dp4a.  Rows that are not 4-byte
@@ -82,13 +153,11 @@ __global__ void __launch_bounds__(256) i8_dp4a_kernel(I8Product p) {
 
 int launch_quantize_tokens(const void* x, int type, long long ld_x, int8_t* q, long long ld_q, float* scale, long long rows, int K,
                            cudaStream_t st) {
-    const dim3 grid(static_cast<unsigned>(rows));
     switch (type) {
-        case kTypeF32: quantize_tokens_kernel<float><<<grid, 128, 0, st>>>(static_cast<const float*>(x), ld_x, q, ld_q, scale, K); break;
-        case kTypeF16: quantize_tokens_kernel<__half><<<grid, 128, 0, st>>>(static_cast<const __half*>(x), ld_x, q, ld_q, scale, K); break;
-        default: quantize_tokens_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(static_cast<const __nv_bfloat16*>(x), ld_x, q, ld_q, scale, K);
+        case kTypeF32: return launch_quantize_t(static_cast<const float*>(x), ld_x, q, ld_q, scale, rows, K, st);
+        case kTypeF16: return launch_quantize_t(static_cast<const __half*>(x), ld_x, q, ld_q, scale, rows, K, st);
+        default: return launch_quantize_t(static_cast<const __nv_bfloat16*>(x), ld_x, q, ld_q, scale, rows, K, st);
     }
-    return cudaGetLastError() == cudaSuccess ? ST_OK : ST_LAUNCH;
 }
 
 int launch_i8_dp4a(const I8Product& p, cudaStream_t st) {

@@ -6,15 +6,15 @@
 // TMEM, so splitting K changes nothing; each output sees one epilogue.
 //
 // Both operands are K-major int8 tiles of 128 bytes of K per stage (128-byte swizzle), pulled in by TMA; rows and K beyond the
-// tensors read as zeros.  Warp 0 = TMA, warp 1 = MMA issue and TMEM owner, warps 2 - 9 = epilogue (two per TMEM lane quarter).
+// tensors read as zeros.  Warp 0 = TMA, warp 1 = MMA issue and TMEM owner, warps 2 - 17 = epilogue (four per TMEM lane quarter).
 #include "i8_common.cuh"
 #include "tma_host.h"
 
 namespace ppml_b200 {
 namespace {
 
-constexpr int kThreadsI8 = 320;
-constexpr int kFirstEpi = 2, kEpiWarps = 8;
+constexpr int kFirstEpi = 2, kEpiWarps = 16, kEpiParts = kEpiWarps / 4;
+constexpr int kThreadsI8 = 32 * (kFirstEpi + kEpiWarps);
 constexpr int kMaxStages = 8;
 constexpr int kRowsA = 128;                        // channels per CTA
 constexpr int kABytes = kRowsA * 128;
@@ -40,8 +40,8 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-__device__ __forceinline__ int ld_cluster_s32(uint32_t cluster_addr) {
-    int v; asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory"); return v;
+__device__ __forceinline__ uint32_t ld_cluster_s32(uint32_t cluster_addr) {
+    uint32_t v; asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory"); return v;
 }
 
 // ---- the forms that a pair of CTAs uses ----
@@ -81,42 +81,47 @@ template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
 }
 
 // ---- epilogue of 32 tokens x this lane's channel ----
-template <typename T>
-__device__ __forceinline__ void store_chunk(const I8Product& p, const int (&sum)[32], float* scale_buf, long long t0, int left, long long n,
-                                            bool n_ok, float b_scale, float bias, int lane) {
-    // left = tokens of the chunk that exist (may be <= 0)
-    __syncwarp();
-    scale_buf[lane] = lane < left ? p.a_scale[t0 + lane] : 0.0f;
-    __syncwarp();
-    if (!n_ok) return;
-    T* c = static_cast<T*>(p.C) + t0 * p.ldc + n;
-    const T* g = static_cast<const T*>(p.gate) + t0 * p.ld_gate + n;
+// FULL: all 32 tokens exist (no branch per token).  `scale` is lane j's token scale; c and g point at the first token's output
+// and gate in this lane's channel.
+template <typename T, bool FULL>
+__device__ __forceinline__ void store_tokens(const I8Product& p, const uint32_t (&sum)[32], const float* scale_buf, int left, T* c, const T* g,
+                                             float b_scale, float bias) {
 #pragma unroll
     for (int j0 = 0; j0 < 32; j0 += 8) {
-        float y[8];
+        if (!FULL && j0 >= left) return;
+        float y[8], s[8];
+        *reinterpret_cast<float4*>(s) = reinterpret_cast<const float4*>(scale_buf)[j0 / 4];
+        *reinterpret_cast<float4*>(s + 4) = reinterpret_cast<const float4*>(scale_buf)[j0 / 4 + 1];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const float4 s = reinterpret_cast<const float4*>(scale_buf)[j0 / 4 + q];
-            y[4 * q] = fmaf(static_cast<float>(sum[j0 + 4 * q]) * s.x, b_scale, bias);
-            y[4 * q + 1] = fmaf(static_cast<float>(sum[j0 + 4 * q + 1]) * s.y, b_scale, bias);
-            y[4 * q + 2] = fmaf(static_cast<float>(sum[j0 + 4 * q + 2]) * s.z, b_scale, bias);
-            y[4 * q + 3] = fmaf(static_cast<float>(sum[j0 + 4 * q + 3]) * s.w, b_scale, bias);
-        }
-        if (p.act != 0) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = i8_act(p.act, y[j]);
-        }
+        for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(static_cast<int>(sum[j0 + j])) * s[j], b_scale, bias);
+        if (p.act != 0) i8_act_all(p.act, y);
         if (p.gate) {
             float gv[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) gv[j] = j0 + j < left ? to_f32(g[(j0 + j) * p.ld_gate]) : 0.0f;
+            for (int j = 0; j < 8; ++j) { gv[j] = FULL || j0 + j < left ? to_f32(*g) : 0.0f; g += p.ld_gate; }
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] *= gv[j];
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j0 + j < left) c[(j0 + j) * p.ldc] = from_f32<T>(y[j]);
+        for (int j = 0; j < 8; ++j) {
+            if (FULL || j0 + j < left) *c = from_f32<T>(y[j]);
+            c += p.ldc;
+        }
     }
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(const I8Product& p, const uint32_t (&sum)[32], float* scale_buf, float scale, long long t0, int left,
+                                            long long n, bool n_ok, float b_scale, float bias, int lane) {
+    __syncwarp();
+    scale_buf[lane] = scale;
+    __syncwarp();
+    if (n_ok) {
+        T* c = static_cast<T*>(p.C) + t0 * p.ldc + n;
+        const T* g = p.gate ? static_cast<const T*>(p.gate) + t0 * p.ld_gate + n : nullptr;
+        if (left >= 32) store_tokens<T, true>(p, sum, scale_buf, left, c, g, b_scale, bias);
+        else store_tokens<T, false>(p, sum, scale_buf, left, c, g, b_scale, bias);
+    }
+    __syncwarp();
 }
 
 // On an abort the copies that are still on their way must not land in the shared memory of a later block.
@@ -233,27 +238,33 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             const bool n_ok = n < q.p.N;
             const float bs = n_ok ? q.p.b_scale[n] : 0.0f, bias = n_ok && q.p.bias ? q.p.bias[n] : 0.0f;
             const long long t0 = static_cast<long long>(tt) * q.bn;
+            const long long rest = q.p.M - t0;
+            const int cols = static_cast<int>(rest < q.bn ? rest : q.bn);
+            float scale[2];                        // of the chunks this warp will read, requested before the wait
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int c = (part + k * kEpiParts) * 32 + lane;
+                scale[k] = c < cols ? q.p.a_scale[t0 + c] : 0.0f;
+            }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull(acc), aph, cta_abort, q.err, 0x840 | acc))) break;
             tc_fence_after();
             const uint32_t d = tmem + acc * (q.tmem_cols / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
-            const long long rest = q.p.M - t0;
-            const int cols = static_cast<int>(rest < q.bn ? rest : q.bn);
-            for (int c = part * 32; c < cols; c += 64) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int c = (part + k * kEpiParts) * 32;
                 uint32_t r[32];
-                __syncwarp();
-                tmem_ld32(d + c, r);
-                tmem_ld_wait();
-                if (c + 64 >= cols) {              // the last read of this warp: the accumulator may be written again
+                if (c < cols) {
+                    __syncwarp();
+                    tmem_ld32(d + c, r);
+                    tmem_ld_wait();
+                }
+                // the last read of this warp, or none in this tile: the accumulator may be written again
+                if (k == (part * 32 + 32 * kEpiParts < cols ? 1 : 0)) {
                     tc_fence_before();
+                    __syncwarp();
                     if (lane == 0) { if (CG == 2) mbar_arrive_cluster(map_to(tempty(acc), 0)); else mbar_arrive(tempty(acc)); }
                 }
-                int v[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = static_cast<int>(r[j]);
-                store_chunk<T>(q.p, v, scale_buf, t0 + c, min(32, cols - c), n, n_ok, bs, bias, lane);
-            }
-            if (part * 32 >= cols && lane == 0) {  // nothing to read in this tile
-                if (CG == 2) mbar_arrive_cluster(map_to(tempty(acc), 0)); else mbar_arrive(tempty(acc));
+                if (c < cols) store_chunk<T>(q.p, r, scale_buf, scale[k], t0 + c, cols - c, n, n_ok, bs, bias, lane);
             }
             if (++acc == 2) { acc = 0; aph ^= 1u; }
         }
@@ -345,23 +356,22 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     const bool n_ok = n < q.p.N;
     const float bs = n_ok ? q.p.b_scale[n] : 0.0f, bias = n_ok && q.p.bias ? q.p.bias[n] : 0.0f;
     float* scale_buf = scales + (warp - kFirstEpi) * 32;
+    const float scale = warp >= kFirstEpi && part * 32 + lane < cols ? q.p.a_scale[t0 + part * 32 + lane] : 0.0f;
     if (warp >= kFirstEpi) {
         if (__all_sync(0xffffffffu, mbar_wait(tfull, 0, cta_abort, q.err, 0x940))) {
             tc_fence_after();
-            for (int c = part * 32; c < cols; c += 64) {
+            const int c = part * 32;               // bn <= 128: at most one chunk per warp
+            if (c < cols) {
                 uint32_t r[32];
                 __syncwarp();
                 tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
                 tmem_ld_wait();
-                int v[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = static_cast<int>(r[j]);
                 if (parts == 1) {
-                    store_chunk<T>(q.p, v, scale_buf, t0 + c, min(32, cols - c), n, n_ok, bs, bias, lane);
+                    store_chunk<T>(q.p, r, scale_buf, scale, t0 + c, cols - c, n, n_ok, bs, bias, lane);
                 } else {                           // the stages are free: every load has landed and every MMA has read
-                    int* buf = reinterpret_cast<int*>(gen) + c * kRowsA + quarter * 32 + lane;
+                    uint32_t* buf = reinterpret_cast<uint32_t*>(gen) + c * kRowsA + quarter * 32 + lane;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) buf[j * kRowsA] = v[j];
+                    for (int j = 0; j < 32; ++j) buf[j * kRowsA] = r[j];
                 }
             }
         }
@@ -370,20 +380,19 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         __syncwarp();
         cluster_sync_all();
         if (warp >= kFirstEpi) {
-            // tokens in chunks of 8, chunk u to the CTA u mod parts, alternating between the two halves of the warps
-            int turn = 0;
-            for (int c = rank * 8; c < cols; c += 8 * parts, turn ^= 1) {
-                if (turn != part) continue;
-                int v[32];
+            // tokens in chunks of 8, dealt to the CTAs and within a CTA to its four groups of warps
+            for (int c = (rank + part * parts) * 8; c < cols; c += 8 * parts * kEpiParts) {
+                uint32_t v[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = 0;
+                const float s = lane < min(8, cols - c) ? q.p.a_scale[t0 + c + lane] : 0.0f;
                 const uint32_t at = base + static_cast<uint32_t>((c * kRowsA + quarter * 32 + lane) * 4);
                 for (int r = 0; r < parts; ++r) {
                     const uint32_t there = map_to(at, static_cast<uint32_t>((rank + r) % parts));
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] += ld_cluster_s32(there + j * kRowsA * 4);
                 }
-                store_chunk<T>(q.p, v, scale_buf, t0 + c, min(8, cols - c), n, n_ok, bs, bias, lane);
+                store_chunk<T>(q.p, v, scale_buf, s, t0 + c, min(8, cols - c), n, n_ok, bs, bias, lane);
             }
         }
     }
