@@ -37,8 +37,10 @@ __device__ __forceinline__ uint32_t map_to(uint32_t saddr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Orders nothing but the tensor memory reads that tcgen05.fence::before_thread_sync put before it: a release at cluster scope
+// would make the warp wait for its stores of results every time (it took a third of the epilogue).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ uint32_t ld_cluster_s32(uint32_t cluster_addr) {
     uint32_t v; asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory"); return v;
@@ -81,30 +83,45 @@ template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
 }
 
 // ---- epilogue of 32 tokens x this lane's channel ----
-// FULL: all 32 tokens exist (no branch per token).  `scale` is lane j's token scale; c and g point at the first token's output
-// and gate in this lane's channel.
-template <typename T, bool FULL>
-__device__ __forceinline__ void store_tokens(const I8Product& p, const uint32_t (&sum)[32], const float* scale_buf, int left, T* c, const T* g,
-                                             float b_scale, float bias) {
+// All 32 tokens, no activation, no gate: straight code, the row pitch in 32 bits (one multiply-add per address).
+template <typename T>
+__device__ __forceinline__ void store_plain(const uint32_t (&sum)[32], const float* scale_buf, T* c, uint32_t ldc, float b_scale, float bias) {
+#pragma unroll
+    for (int j0 = 0; j0 < 32; j0 += 4) {
+        const float4 s = reinterpret_cast<const float4*>(scale_buf)[j0 / 4];
+        const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            c[static_cast<uint64_t>(ldc) * static_cast<uint32_t>(j0 + j)] =
+                from_f32<T>(fmaf(static_cast<float>(static_cast<int>(sum[j0 + j])) * f[j], b_scale, bias));
+    }
+}
+// Everything else.
+template <typename T>
+__device__ __forceinline__ void store_any(const I8Product& p, const uint32_t (&sum)[32], const float* scale_buf, int left, T* c, const T* g,
+                                       float b_scale, float bias) {
 #pragma unroll
     for (int j0 = 0; j0 < 32; j0 += 8) {
-        if (!FULL && j0 >= left) return;
+        if (j0 >= left) return;
         float y[8], s[8];
         *reinterpret_cast<float4*>(s) = reinterpret_cast<const float4*>(scale_buf)[j0 / 4];
         *reinterpret_cast<float4*>(s + 4) = reinterpret_cast<const float4*>(scale_buf)[j0 / 4 + 1];
 #pragma unroll
         for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(static_cast<int>(sum[j0 + j])) * s[j], b_scale, bias);
-        if (p.act != 0) i8_act_all(p.act, y);
-        if (p.gate) {
+        if (p.act != 0) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) *reinterpret_cast<float4*>(y + j) = i8_act4(p.act, make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]));
+        }
+        if (g) {
             float gv[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { gv[j] = FULL || j0 + j < left ? to_f32(*g) : 0.0f; g += p.ld_gate; }
+            for (int j = 0; j < 8; ++j) { gv[j] = j0 + j < left ? to_f32(*g) : 0.0f; g += p.ld_gate; }
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] *= gv[j];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (FULL || j0 + j < left) *c = from_f32<T>(y[j]);
+            if (j0 + j < left) *c = from_f32<T>(y[j]);
             c += p.ldc;
         }
     }
@@ -117,9 +134,8 @@ __device__ __forceinline__ void store_chunk(const I8Product& p, const uint32_t (
     __syncwarp();
     if (n_ok) {
         T* c = static_cast<T*>(p.C) + t0 * p.ldc + n;
-        const T* g = p.gate ? static_cast<const T*>(p.gate) + t0 * p.ld_gate + n : nullptr;
-        if (left >= 32) store_tokens<T, true>(p, sum, scale_buf, left, c, g, b_scale, bias);
-        else store_tokens<T, false>(p, sum, scale_buf, left, c, g, b_scale, bias);
+        if (left >= 32 && p.act == 0 && !p.gate && p.ldc <= 0x7fffffffLL) store_plain<T>(sum, scale_buf, c, static_cast<uint32_t>(p.ldc), b_scale, bias);
+        else store_any<T>(p, sum, scale_buf, left, c, p.gate ? static_cast<const T*>(p.gate) + t0 * p.ld_gate + n : nullptr, b_scale, bias);
     }
     __syncwarp();
 }
