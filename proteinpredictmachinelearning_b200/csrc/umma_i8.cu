@@ -16,6 +16,7 @@ namespace {
 constexpr int kFirstEpi = 2, kEpiWarps = 16, kEpiParts = kEpiWarps / 4;
 constexpr int kThreadsI8 = 32 * (kFirstEpi + kEpiWarps);
 constexpr int kMaxStages = 8;
+constexpr int kSmemMax = 227 * 1024;
 constexpr int kRowsA = 128;                        // channels per CTA
 constexpr int kABytes = kRowsA * 128;
 constexpr int kBarBytes = 256, kScaleBytes = kEpiWarps * 32 * 4;
@@ -80,6 +81,26 @@ template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
     else
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                      ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+
+// One stage: up to four MMAs of 32 k and the commit that hands the stage back.  The whole warp walks the loops around this with
+// uniform values and one elected lane issues: descriptors then stay in uniform registers (inside a branch taken by lane 0
+// alone, the four MMAs took 540 cycles to issue, longer than the 512 they run).
+template <int CG>
+__device__ __forceinline__ void issue_block(bool lead, uint32_t d, uint64_t desc_a, uint32_t idesc, int steps, uint32_t accumulate, uint32_t empty) {
+    const uint64_t desc_b = desc_a + (kABytes >> 4);
+    if (lead) {
+        if (steps == 4) {
+            mma_i8<CG>(d, desc_a, desc_b, idesc, accumulate);
+            mma_i8<CG>(d, desc_a + 2, desc_b + 2, idesc, 1u);
+            mma_i8<CG>(d, desc_a + 4, desc_b + 4, idesc, 1u);
+            mma_i8<CG>(d, desc_a + 6, desc_b + 6, idesc, 1u);
+        } else {
+            for (int k = 0; k < steps; ++k) mma_i8<CG>(d, desc_a + 2 * k, desc_b + 2 * k, idesc, k == 0 ? accumulate : 1u);
+        }
+        commit<CG>(empty);
+    }
+    __syncwarp();
 }
 
 // ---- epilogue of 32 tokens x this lane's channel ----
@@ -152,9 +173,9 @@ __device__ __noinline__ void wait_for_copies() {
 template <typename T, int CG>
 __global__ void __launch_bounds__(kThreadsI8, 1)
 i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const I8Tc q) {
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    extern __shared__ __align__(1024) uint8_t smem_raw[];      // no static shared memory: it starts on the swizzle's 1024 bytes
+    const uint32_t base = smem_u32(smem_raw);
+    uint8_t* gen = smem_raw;
     const uint32_t bars = base + q.stages * q.stage_bytes;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
@@ -221,26 +242,26 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             const uint32_t idesc = make_idesc(2, 1, 1, 0, 0, kRowsA * CG, q.bn);
             const int last_steps = (q.p.K - (q.kblocks - 1) * 128 + 31) / 32;
+            const uint64_t desc0 = make_smem_desc(base, 16, 1024, kLayoutSW128);
+            const uint32_t step = static_cast<uint32_t>(q.stage_bytes) >> 4;
+            const bool lead = elect_one();
             int s = 0; uint32_t ph = 0; bool ok = true; int acc = 0; uint32_t aph = 0;
             for (int i = group; i < tiles && ok; i += groups) {
-                if (!mbar_wait(tempty(acc), aph ^ 1u, cta_abort, q.err, 0x820 | acc)) break;
+                if (!__all_sync(0xffffffffu, mbar_wait(tempty(acc), aph ^ 1u, cta_abort, q.err, 0x820 | acc))) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * (q.tmem_cols / 2);
                 for (int kb = 0; kb < q.kblocks; ++kb) {
-                    if (!mbar_wait(full(s), ph, cta_abort, q.err, 0x830 | s)) { ok = false; break; }
+                    if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, cta_abort, q.err, 0x830 | s))) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t at = base + s * q.stage_bytes;
-                    const uint64_t da = make_smem_desc(at, 16, 1024, kLayoutSW128), db = make_smem_desc(at + kABytes, 16, 1024, kLayoutSW128);
-                    const int steps = kb == q.kblocks - 1 ? last_steps : 4;
-                    for (int k = 0; k < steps; ++k) mma_i8<CG>(d, da + 2 * k, db + 2 * k, idesc, kb != 0 || k != 0);
-                    commit<CG>(empty(s));
+                    issue_block<CG>(lead, d, desc0 + static_cast<uint64_t>(s * step), idesc, kb == q.kblocks - 1 ? last_steps : 4, kb != 0, empty(s));
                     if (++s == q.stages) { s = 0; ph ^= 1u; }
                 }
                 if (!ok) break;
-                commit<CG>(tfull(acc));
+                if (lead) commit<CG>(tfull(acc));
+                __syncwarp();
                 if (++acc == 2) { acc = 0; aph ^= 1u; }
             }
         }
@@ -300,9 +321,9 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
 template <typename T>
 __global__ void __launch_bounds__(kThreadsI8, 1)
 i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const I8Tc q, const int parts) {
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+    extern __shared__ __align__(1024) uint8_t smem_raw[];      // no static shared memory: it starts on the swizzle's 1024 bytes
+    const uint32_t base = smem_u32(smem_raw);
+    uint8_t* gen = smem_raw;
     const uint32_t bars = base + q.stages * q.stage_bytes;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
@@ -349,22 +370,19 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = make_idesc(2, 1, 1, 0, 0, kRowsA, q.bn);
-            const int last_steps = (q.p.K - (q.kblocks - 1) * 128 + 31) / 32;
-            int s = 0; uint32_t ph = 0; bool ok = true;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(full(s), ph, cta_abort, q.err, 0x930 | s)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t at = base + s * q.stage_bytes;
-                const uint64_t da = make_smem_desc(at, 16, 1024, kLayoutSW128), db = make_smem_desc(at + kABytes, 16, 1024, kLayoutSW128);
-                const int steps = kb == q.kblocks - 1 ? last_steps : 4;
-                for (int k = 0; k < steps; ++k) umma<MmaKind::I8>(tmem, da + 2 * k, db + 2 * k, idesc, kb != kb0 || k != 0);
-                umma_commit(empty(s));
-                if (++s == q.stages) { s = 0; ph ^= 1u; }
-            }
-            if (ok) umma_commit(tfull);
+        const uint32_t idesc = make_idesc(2, 1, 1, 0, 0, kRowsA, q.bn);
+        const int last_steps = (q.p.K - (q.kblocks - 1) * 128 + 31) / 32;
+        const uint64_t desc0 = make_smem_desc(base, 16, 1024, kLayoutSW128);
+        const uint32_t step = static_cast<uint32_t>(q.stage_bytes) >> 4;
+        const bool lead = elect_one();
+        int s = 0; uint32_t ph = 0; bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!__all_sync(0xffffffffu, mbar_wait(full(s), ph, cta_abort, q.err, 0x930 | s))) { ok = false; break; }
+            tc_fence_after();
+            issue_block<1>(lead, tmem, desc0 + static_cast<uint64_t>(s * step), idesc, kb == q.kblocks - 1 ? last_steps : 4, kb != kb0, empty(s));
+            if (++s == q.stages) { s = 0; ph ^= 1u; }
         }
+        if (ok && lead) umma_commit(tfull);
     }
     __syncwarp();
     const int quarter = warp & 3, part = (warp - kFirstEpi) >> 2;
@@ -426,7 +444,7 @@ int pow2_at_least(int v, int lo) { int c = lo; while (c < v) c *= 2; return c; }
 
 template <typename... KArgs, typename... Args>
 cudaError_t launch_cluster(void (*kernel)(KArgs...), int grid, int cluster, size_t smem, cudaStream_t st, Args... args) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kThreadsI8); cfg.dynamicSmemBytes = smem; cfg.stream = st;
@@ -467,7 +485,7 @@ int launch_t(const I8Product& p, const Plan& plan, cudaStream_t st) {
     I8Tc q{};
     q.p = p; q.bn = plan.bn;
     q.stage_bytes = kABytes + plan.bn / cg * 128;
-    q.stages = 200 * 1024 / q.stage_bytes;
+    q.stages = (kSmemMax - kBarBytes - kScaleBytes) / q.stage_bytes;
     if (q.stages > kMaxStages) q.stages = kMaxStages;
     q.kblocks = (p.K + 127) / 128;
     q.tiles_n = static_cast<int>((p.N + static_cast<long long>(kRowsA) * cg - 1) / (kRowsA * cg));
@@ -479,7 +497,7 @@ int launch_t(const I8Product& p, const Plan& plan, cudaStream_t st) {
     if (!make_tmap_3d(&tmW, TmaType::U8, p.B, p.K, p.N, 1, p.ldb, 0, 128, kRowsA, 1) ||
         !make_tmap_3d(&tmA, TmaType::U8, p.A, p.K, p.M, 1, p.lda, 0, 128, plan.bn / cg, 1))
         return ST_UNSUPPORTED_PATH;
-    const size_t smem = static_cast<size_t>(q.stages) * q.stage_bytes + kBarBytes + kScaleBytes + 1024;
+    const size_t smem = static_cast<size_t>(q.stages) * q.stage_bytes + kBarBytes + kScaleBytes;
     cudaError_t e;
     if (plan.pair == 0) {
         q.tmem_cols = pow2_at_least(plan.bn, 32);
