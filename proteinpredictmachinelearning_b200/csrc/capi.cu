@@ -332,7 +332,7 @@ int ppml_b200_mul_mat_i8(const int8_t* A, int64_t lda, const float* a_scale, con
 }
 
 int64_t ppml_b200_linear_i8_workspace(int64_t M, int K) {
-    return M <= 0 || K <= 0 ? 0 : M * round16(K) + round16(4 * M);
+    return M <= 0 || K <= 0 || i8_few(M, K) ? 0 : M * round16(K) + round16(4 * M);
 }
 
 int ppml_b200_linear_i8(const void* X, int x_type, int64_t ld_x, const int8_t* B, int64_t ldb, const float* b_scale, void* C,
@@ -343,6 +343,10 @@ int ppml_b200_linear_i8(const void* X, int x_type, int64_t ld_x, const int8_t* B
     if (!type_ok(x_type) || ld_x < K || !aligned(bias, 4)) return ST_BAD_ARGS;
     if (M == 0) return ST_OK;
     if (!X || !aligned(X, type_bytes(x_type))) return ST_BAD_ARGS;
+    if (i8_few(M, K)) {
+        if (path == PPML_B200_PATH_UMMA) return ST_UNSUPPORTED_PATH;
+        return launch_i8_few(X, x_type, ld_x, I8Product{nullptr, B, 0, ldb, nullptr, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act}, as_stream(stream));
+    }
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < ppml_b200_linear_i8_workspace(M, K)) return ST_SCRATCH;
     int8_t* q = static_cast<int8_t*>(workspace);
     const int64_t ld = round16(K);

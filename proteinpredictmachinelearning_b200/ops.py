@@ -243,8 +243,7 @@ def quantize_tokens_i8(x, out=None):
             return quantize_tokens_i8(x, out)
     ld = _pitch(x, x.dtype, M, K, dev, "x")
     if out is None:
-        q = torch.empty((M, (K + 15) & -16), device=dev, dtype=torch.int8)
-        out = (q if q.shape[1] == K else q[:, :K], torch.empty(M, device=dev, dtype=torch.float32))
+        out = (torch.empty_strided((M, K), ((K + 15) & -16, 1), device=dev, dtype=torch.int8), torch.empty_strided((M,), (1,), device=dev, dtype=torch.float32))
     q, scale = out
     rc = _lib.load().ppml_b200_quantize_tokens_i8(x.data_ptr(), TYPE[x.dtype], ld, q.data_ptr(), _pitch(q, torch.int8, M, K, dev, "q"),
                                                   _vec(scale, M, dev, "scale"), M, K, _raw_stream(dev))
@@ -262,7 +261,7 @@ def _product_args(dev, M, K, W, w_scale, bias, gate, act, dtype, path, out):
     N = W.shape[0]
     ldb = _pitch(W, torch.int8, N, K, dev, "W")
     if out is None:
-        out, ldc = torch.empty((M, N), device=dev, dtype=dtype), N
+        out, ldc = torch.empty_strided((M, N), (N, 1), device=dev, dtype=dtype), N      # half the time of torch.empty
     else:
         ldc = _pitch(out, dtype, M, N, dev, "out")
     g, ldg = (None, 0) if gate is None else (gate.data_ptr(), _pitch(gate, dtype, M, N, dev, "gate"))
@@ -303,7 +302,7 @@ def linear_i8(x, W, w_scale, bias=None, gate=None, act="none", dtype=None, path=
     ld = _pitch(x, x.dtype, M, K, dev, "x")
     out, args = _product_args(dev, M, K, W, w_scale, bias, gate, act, out.dtype if out is not None else dtype or x.dtype, path, out)
     need = lib.ppml_b200_linear_i8_workspace(M, K)
-    ws = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    ws = torch.empty_strided((need,), (1,), device=dev, dtype=torch.uint8) if need else None
     rc = lib.ppml_b200_linear_i8(x.data_ptr(), TYPE[x.dtype], ld, *args, None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
     if rc:
         _check(rc, "linear_i8")

@@ -113,7 +113,7 @@ def test_quantizer_ties_zeros_and_extremes(K, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("M", [6, 70])
+@pytest.mark.parametrize("M", [5, 70])
 def test_rows_with_infinities_or_nan_give_nan_and_leave_the_others(dtype, M, no_device_abort):
     x = rows(M, 272, dtype, 3)
     x[1, 7], x[2, 0], x[4, 271] = float("nan"), float("inf"), float("-inf")
@@ -125,6 +125,8 @@ def test_rows_with_infinities_or_nan_give_nan_and_leave_the_others(dtype, M, no_
         y = ops.linear_i8(x, W, ws, dtype=F32, path=path)
         assert torch.isnan(y[bad]).all()
         check_product(y[~bad], q[~bad], s[~bad], W, ws, None, None, "none")
+        few = ops.linear_i8(x[:4], W, ws, dtype=F32, path=path)
+        assert torch.isnan(few[1:3]).all() and torch.equal(few[0], y[0]) and torch.equal(few[3], y[3])
 
 
 @gpu
@@ -225,7 +227,7 @@ def test_largest_sums_are_exact(M, N, no_device_abort):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_linear_is_quantizer_and_product(M, dtype, no_device_abort):
     """One call, two calls, the CUDA-core path and any part of the tokens give the same bits."""
-    for K, N in ((272, 200), (100, 64), (2049, 72)):
+    for K, N in ((272, 200), (100, 64), (2049, 72), (528, 3500), (5000, 9), (34000, 24)):
         x = rows(M, K, dtype, M, K + 8)
         W, ws = ops.quantize_tokens_i8(rows(N, K, F32, 9) * 0.02)
         bias = scales(N, 5)
@@ -236,6 +238,11 @@ def test_linear_is_quantizer_and_product(M, dtype, no_device_abort):
         assert torch.equal(y, ops.mul_mat_i8(q, s, W, ws, bias=bias, dtype=dtype))
         assert torch.equal(y, ops.linear_i8(x, W, ws, bias=bias, path=PATH_SIMT))
         assert torch.equal(y[M // 2:], ops.linear_i8(x[M // 2:], W, ws, bias=bias))
+    x, W = rows(M, 272, dtype, 1, 275, 3), ints(90, 272, 2, 273, 1)           # nothing on 16 bytes
+    gate = rows(M, 90, F32, 4)
+    y = ops.linear_i8(x, W, scales(90, 2), gate=gate, act="gelu", dtype=F32)
+    q, s = ops.quantize_tokens_i8(x)
+    check_product(y, q, s, W, scales(90, 2), None, gate, "gelu")
 
 
 @gpu
@@ -339,15 +346,16 @@ def test_bad_arguments_are_refused_on_the_host(lib):
     assert mm(M=0) == 0 and mm(M=0, A=None, C=None, a_scale=None) == 0
     assert mm(path=2, A=C.c_void_p(68)) == 7 and mm(path=2, lda=17) == 7 and mm(path=2, B=C.c_void_p(72)) == 7 and mm(path=2, ldb=24) == 7
 
-    assert lib.ppml_b200_linear_i8_workspace(3, 17) == 3 * 32 + 16 and lib.ppml_b200_linear_i8_workspace(0, 17) == 0
+    assert lib.ppml_b200_linear_i8_workspace(5, 17) == 5 * 32 + 32 and lib.ppml_b200_linear_i8_workspace(0, 17) == 0
+    assert lib.ppml_b200_linear_i8_workspace(4, 17) == 0 and lib.ppml_b200_linear_i8_workspace(4, 32769) == 4 * 32784 + 16
     names = ("X", "x_type", "ld_x", "B", "ldb", "b_scale", "C", "ldc", "c_type", "M", "K", "N", "bias", "gate", "ld_gate", "act", "path", "ws", "bytes")
-    good = (p, 0, 16, p, 16, p, p, 8, 0, 4, 16, 8, None, None, 0, 0, 0, p, 80)
+    good = (p, 0, 16, p, 16, p, p, 8, 0, 6, 16, 8, None, None, 0, 0, 0, p, 128)
 
     def lin(**kw):
         return lib.ppml_b200_linear_i8(*[kw.get(n, v) for n, v in zip(names, good)], None)
     for bad in (dict(X=None), dict(x_type=3), dict(ld_x=15), dict(X=C.c_void_p(66)), dict(B=None), dict(N=0), dict(act=9)):
         assert lin(**bad) == 1, bad
-    assert lin(ws=None) == 3 and lin(bytes=79) == 3 and lin(ws=C.c_void_p(72)) == 3
+    assert lin(ws=None) == 3 and lin(bytes=127) == 3 and lin(M=4, path=2) == 7 and lin(ws=C.c_void_p(72)) == 3
     assert lin(M=0, ws=None, bytes=0) == 0 and lin(K=131072, ldb=1 << 18, ld_x=1 << 18) == 9
 
 

@@ -226,6 +226,23 @@ def test_infinities_and_nan_stay_in_their_row(dtype, no_device_abort):
 
 
 @gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rot", [(64, 16), (32, 0), (40, 4), (33, 10), (64, 12)])
+def test_infinities_and_nan_stay_in_their_pair_without_a_norm(d, rot, interleaved, no_device_abort):
+    """Without a norm a value meets its partner of the rotation and nothing else, forward and backward."""
+    q = rand((2, 3, 2, d), 1)
+    cos, sin = ops.rope_table(3, rot) if rot else (None, None)
+    for e, value in ((rot, float("inf")), (d - 1, float("nan")), (rot + 1, float("-inf"))):
+        x = q.clone()
+        x[0, 2, 1, e] = value
+        y, _ = ops.qk_norm_rope(x, None, norm="none", cos=cos, sin=sin, interleaved=interleaved)
+        g = ops.qk_norm_rope_backward(q, None, x, None, norm="none", cos=cos, sin=sin, interleaved=interleaved)["dQ"]
+        for r in (y, g):
+            finite = torch.isfinite(r)
+            assert not finite[0, 2, 1, e] and int((~finite).sum()) == 1
+
+
+@gpu
 @pytest.mark.parametrize("d", [64, 40, 33])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_positions_padding_and_the_end_of_the_table(d, dtype, no_device_abort):
