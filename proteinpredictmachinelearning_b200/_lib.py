@@ -50,10 +50,10 @@ SIGNATURES = {
     "ppml_b200_mul_mat_i8": (_i, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp]),
     "ppml_b200_linear_i8_workspace": (_i64, [_i64, _i]),
     "ppml_b200_linear_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp, _i64, _vp]),
-    "ppml_b200_qk_norm_rope": (_i, [C.POINTER(QkCfg), C.POINTER(Heads), C.POINTER(Heads)] + [_vp] * 5 + [C.POINTER(Heads)] * 2 + [_vp]),
-    "ppml_b200_qk_norm_rope_backward_workspace": (_i64, [C.POINTER(QkCfg)]),
-    "ppml_b200_qk_norm_rope_backward": (_i, [C.POINTER(QkCfg), C.POINTER(Heads), C.POINTER(Heads)] + [_vp] * 5 + [C.POINTER(Heads)] * 4 +
-                                        [_vp, _vp, _vp, _i64, _vp]),
+    # structures as plain addresses: a caller may pass packed bytes (ops) or byref of the classes above
+    "ppml_b200_qk_norm_rope": (_i, [_vp] * 11),
+    "ppml_b200_qk_norm_rope_backward_workspace": (_i64, [_vp]),
+    "ppml_b200_qk_norm_rope_backward": (_i, [_vp] * 15 + [_i64, _vp]),
     "ppml_b200_quantize_rows_q8_1": (_i, [_vp, _vp, _i64, _vp]),
     "ppml_b200_dequantize_q8_0": (_i, [_vp, _vp, _i64, _vp]),
     "ppml_b200_dequantize_q8_1": (_i, [_vp, _vp, _i64, _vp]),

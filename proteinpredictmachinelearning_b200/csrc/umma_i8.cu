@@ -7,6 +7,8 @@
 //
 // Both operands are K-major int8 tiles of 128 bytes of K per stage (128-byte swizzle), pulled in by TMA; rows and K beyond the
 // tensors read as zeros.  Warp 0 = TMA, warp 1 = MMA issue and TMEM owner, warps 2 - 17 = epilogue (four per TMEM lane quarter).
+#include <atomic>
+
 #include "i8_common.cuh"
 #include "tma_host.h"
 
@@ -442,10 +444,19 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
 
 int pow2_at_least(int v, int lo) { int c = lo; while (c < v) c *= 2; return c; }
 
-template <typename... KArgs, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), int grid, int cluster, size_t smem, cudaStream_t st, Args... args) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+template <auto kernel, typename... Args>
+cudaError_t launch_cluster(int grid, int cluster, size_t smem, cudaStream_t st, const Args&... args) {
+    // the attribute once per kernel and device (two threads may both set it)
+    static std::atomic<uint64_t> allowed{0};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+        if (e != cudaSuccess) return e;
+        allowed.fetch_or(bit, std::memory_order_relaxed);
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kThreadsI8); cfg.dynamicSmemBytes = smem; cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -501,12 +512,12 @@ int launch_t(const I8Product& p, const Plan& plan, cudaStream_t st) {
     cudaError_t e;
     if (plan.pair == 0) {
         q.tmem_cols = pow2_at_least(plan.bn, 32);
-        e = launch_cluster(i8_parts_kernel<T>, q.tiles_n * q.tiles_t * plan.parts, plan.parts, smem, st, tmW, tmA, q, plan.parts);
+        e = launch_cluster<i8_parts_kernel<T>>(q.tiles_n * q.tiles_t * plan.parts, plan.parts, smem, st, tmW, tmA, q, plan.parts);
     } else {
         q.tmem_cols = 2 * pow2_at_least(plan.bn, 32);
         const int units = q.tiles_n * q.tiles_t, most = num_sms() / cg, groups = units < most ? units : most;
-        e = cg == 2 ? launch_cluster(i8_tiles_kernel<T, 2>, groups * 2, 2, smem, st, tmW, tmA, q)
-                    : launch_cluster(i8_tiles_kernel<T, 1>, groups, 1, smem, st, tmW, tmA, q);
+        e = cg == 2 ? launch_cluster<i8_tiles_kernel<T, 2>>(groups * 2, 2, smem, st, tmW, tmA, q)
+                    : launch_cluster<i8_tiles_kernel<T, 1>>(groups, 1, smem, st, tmW, tmA, q);
     }
     if (e != cudaSuccess) { cudaGetLastError(); return ST_LAUNCH; }
     return ST_OK;

@@ -517,6 +517,15 @@ def test_bad_arguments_are_refused_on_the_host(lib):
     assert fwd(dict(B=0), Q=None, K=None, Qo=None, Ko=None) == 0 and bwd(dict(L=0), Q=None, K=None, Qo=None, Ko=None, dQ=None, dK=None) == 0
 
 
+def test_packed_structures_are_the_librarys():
+    """ops packs the structures itself: same size and fields as the ctypes classes."""
+    cfg = _lib.QkCfg.from_buffer_copy(ops._QK_CFG.pack(*range(1, 8), 0.5, 9, 10, 11, -(1 << 40)))
+    assert C.sizeof(_lib.QkCfg) == ops._QK_CFG.size
+    assert [getattr(cfg, n) for n, _ in _lib.QkCfg._fields_] == [1, 2, 3, 4, 5, 6, 7, 0.5, 9, 10, 11, -(1 << 40)]
+    v = _lib.Heads.from_buffer_copy(ops._HEADS.pack(1 << 50, 2, -3, 1 << 41))
+    assert C.sizeof(_lib.Heads) == ops._HEADS.size and (v.p, v.sb, v.sl, v.sh) == (1 << 50, 2, -3, 1 << 41)
+
+
 def test_rope_table_in_64_bits():
     cos, sin = ops.rope_table(70000, 64, base=500.0, device="cpu")
     p, i = 69999, np.arange(32)
