@@ -20,16 +20,17 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// The work of a side in the vector kernels: batches of rows per warp, and the steps (tokens, heads) from a batch's row to its next
-// and from a warp's batch to its next.
-struct QkStep { long long batches, warps; uint32_t jump_t; int jump_h; uint32_t sub_t; int sub_h; };
+// What the vector kernels need: byte strides in 32 bits, and how a side's heads are cut into work items.
+struct QkView { unsigned char* p; uint32_t b, l, h; };
+struct QkSide { QkView x, y, dx; const float* w; int H, per_item, chunks; uint32_t items, blocks, chunks_mul; int chunks_shift; };
 struct QkVec {
-    QkParams p;
+    QkSide side[2];                                // Q, K
+    const float* cos_t; const float* sin_t; const int* positions; float* partial;
+    long long pos_b;
+    uint32_t L, l_mul; int l_shift;                // division by L
+    int d, rot, norm, interleaved, table_rows, table_vec, all_turn;
     int G;                                         // lanes per row
-    unsigned blocks_q;                             // blocks on Q's rows; the others are on K's
-    QkStep step_q, step_k;
-    uint32_t l_mul; int l_shift;                   // division by L
-    int table_vec;                                 // 16-byte reads of the table
+    float eps;
 };
 
 // ---- any head dim, any alignment: one warp per row ----------------------------------------------------------------------
@@ -218,9 +219,12 @@ __global__ void __launch_bounds__(32 * kWarps) qk_backward_kernel(const QkParams
 // ---- vector kernels ----------------------------------------------------------------------------------------------------
 // A lane holds two chunks of V neighbouring values (VB bytes each) that rotate with one another: chunks l and l + rot / 2 / V for
 // the pairs (i, i + rot / 2), chunks 2 l and 2 l + 1 for neighbouring pairs and for dims that pass.  So a rotation needs no
-// exchange between lanes, and the table is read once per pair.  G lanes (a power of two) hold a row, a warp W = 32 / G rows.
-// A block works on one side (Q or K): its weights stay in registers.  Rows are taken in batches of U * W consecutive ones
-// per warp, all of a batch's loads requested before the first is used.
+// exchange between lanes.  G lanes (a power of two) hold a row, a warp 32 / G of them, of different tokens: each group of
+// lanes walks over the heads of its token, so that the position, its table row, the weights and all but one addition of
+// an address are had once per token instead of once per row (20 instructions a value before, 6 now).  A block works on one
+// side (Q or K).  Where there are few tokens the heads are dealt to several items.
+constexpr int kHeadsAtOnce = 4;                    // rows per lane whose loads are in flight together (forward)
+
 template <int VB> struct RawOf;
 template <> struct RawOf<16> { using type = uint4; };
 template <> struct RawOf<8> { using type = uint2; };
@@ -245,249 +249,279 @@ template <typename T, int VB> __device__ __forceinline__ typename RawOf<VB>::typ
 // (n m) >> (32 + s) is exact; d = 1 has m = 0.
 __device__ __forceinline__ uint32_t div_by(uint32_t n, uint32_t m, int s) { return m == 0 ? n : __umulhi(n, m) >> s; }
 
-struct Side { HeadsView x, y, dx; const float* w; int H; };
-__device__ __forceinline__ Side side_of(const QkVec& v, bool key) {
-    const QkParams& p = v.p;
-    return key ? Side{p.k, p.ko, p.dk, p.kw, p.hk} : Side{p.q, p.qo, p.dq, p.qw, p.hq};
+// 1 / sqrt(v): the hardware's estimate and one Newton step (within 1 unit in the last place; a division and a square root
+// take 40 instructions).  0 and infinity stay what the estimate makes of them.
+__device__ __forceinline__ float inv_sqrt(float v) {
+    const float r = rsqrtf(v);
+    return r > 0.0f && r < __uint_as_float(0x7f800000u) ? fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r) : r;
 }
 
 // This lane's part of a row and where its pair stands in the table.
-template <int V> struct Lane { int a, b, pair; bool has_a, has_b, turns; };
-template <int V> __device__ __forceinline__ Lane<V> lane_of(const QkVec& v, int l) {
-    Lane<V> n;
-    const int chunks = v.p.d / V, half = v.p.interleaved ? 0 : v.p.rot / 2 / V;
-    n.turns = v.p.interleaved ? l * V < v.p.rot / 2 : l < half;
-    n.a = !v.p.interleaved && l < half ? l : 2 * half + 2 * (l - half);
-    n.b = !v.p.interleaved && l < half ? l + half : n.a + 1;
-    n.has_a = n.a < chunks; n.has_b = n.b < chunks;
+struct Lane { uint32_t a, b; int pair; bool has_a, has_b, turns; };      // a, b: elements
+template <int V> __device__ __forceinline__ Lane lane_of(const QkVec& v, int l) {
+    Lane n;
+    const int chunks = v.d / V, half = v.interleaved ? 0 : v.rot / 2 / V;
+    const bool halves = l < half;
+    n.turns = v.interleaved ? l * V < v.rot / 2 : halves;
+    const int a = halves ? l : 2 * half + 2 * (l - half), b = halves ? l + half : a + 1;
+    n.has_a = a < chunks; n.has_b = b < chunks;
     n.pair = l * V;
-    n.a *= V; n.b *= V;
+    n.a = static_cast<uint32_t>(a * V); n.b = static_cast<uint32_t>(b * V);
     return n;
 }
-// cos and sin of the lane's pairs (garbage where none of them turns); NaN beyond the table
-template <int V> __device__ __forceinline__ void load_table(const QkVec& v, const Lane<V>& n, int pos, float (&c)[V], float (&s)[V]) {
-    const int half = v.p.rot / 2;
+// cos and sin of the lane's pairs; NaN beyond the table; 1 and 0 where nothing turns
+template <int V> __device__ __forceinline__ void load_table(const QkVec& v, const Lane& n, int pos, float (&c)[V], float (&s)[V]) {
+    const int half = v.rot / 2;
+    const float none = n.turns && pos >= v.table_rows ? __uint_as_float(0x7fffffffu) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) { c[i] = __uint_as_float(0x7fffffffu); s[i] = 0.0f; }
-    if (!n.turns || pos >= v.p.table_rows) return;
+    for (int i = 0; i < V; ++i) { c[i] = n.pair + i < half ? none : 1.0f; s[i] = 0.0f; }
+    if (!n.turns || pos >= v.table_rows) return;
     const long long at = static_cast<long long>(pos) * half + n.pair;
     if (V % 4 == 0 && v.table_vec) {
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
-            *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(v.p.cos_t + at + i);
-            *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(v.p.sin_t + at + i);
+            *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(v.cos_t + at + i);
+            *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(v.sin_t + at + i);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (n.pair + i < half) { c[i] = v.p.cos_t[at + i]; s[i] = v.p.sin_t[at + i]; }     // neighbours: may end inside the chunk
-    }
-}
-// x[0 .. V) is the first chunk, x[V .. 2 V) the second; SIGN -1 turns back.  Values that do not turn are not touched: an infinity
-// among them must not meet a neighbour, not even times 0.
-template <int V, int SIGN> __device__ __forceinline__ void turn(float (&x)[2 * V], const float (&c)[V], const float (&s)[V], const QkParams& p,
-                                                                const Lane<V>& n) {
-    if (!n.turns) return;
-    if (p.interleaved) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (n.pair + i >= p.rot / 2) break;
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = fmaf(-SIGN * b, s[i], a * c[i]);
-            x[2 * i + 1] = fmaf(SIGN * a, s[i], b * c[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float a = x[i], b = x[V + i];
-            x[i] = fmaf(-SIGN * b, s[i], a * c[i]);
-            x[V + i] = fmaf(SIGN * a, s[i], b * c[i]);
-        }
+            if (n.pair + i < half) { c[i] = v.cos_t[at + i]; s[i] = v.sin_t[at + i]; }     // neighbours: may end inside the chunk
     }
 }
 __device__ __forceinline__ float group_sum(float v, int G) {
     for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// Row t, h of this lane's group and the step to another one.
-struct At { uint32_t t; int h; };
-__device__ __forceinline__ void advance(At& r, uint32_t dt, int dh, int H) {
-    r.t += dt; r.h += dh;
-    if (r.h >= H) { r.h -= H; ++r.t; }
+// Sum over a row, packed pairs of additions inside the lane.
+template <int N> __device__ __forceinline__ float lane_sum(const float (&x)[N]) {
+    if constexpr (N == 2) return x[0] + x[1];
+    uint64_t t = pack2(x[0], x[1]);
+#pragma unroll
+    for (int i = 2; i < N; i += 2) t = fadd2(t, pack2(x[i], x[i + 1]));
+    float a, b; unpack2(t, a, b);
+    return a + b;
+}
+template <int N> __device__ __forceinline__ float lane_dot(const float (&x)[N], const float (&y)[N]) {
+    uint64_t t = fmul2(pack2(x[0], x[1]), pack2(y[0], y[1]));
+#pragma unroll
+    for (int i = 2; i < N; i += 2) t = ffma2(pack2(x[i], x[i + 1]), pack2(y[i], y[i + 1]), t);
+    float a, b; unpack2(t, a, b);
+    return a + b;
+}
+// (x - mean) and 1 / sqrt(..) of a row; values that do not exist stay 0
+template <int V> __device__ __forceinline__ float normalizer(const QkVec& v, const Lane& n, float inv_d, float (&x)[2 * V]) {
+    if (v.norm == 0) return 1.0f;
+    if (v.norm == 2) {
+        const float m = group_sum(lane_sum(x), v.G) * inv_d;
+#pragma unroll
+        for (int i = 0; i < V; ++i) { x[i] = n.has_a ? x[i] - m : 0.0f; x[V + i] = n.has_b ? x[V + i] - m : 0.0f; }
+    }
+    return inv_sqrt(fmaf(group_sum(lane_dot(x, x), v.G), inv_d, v.eps));
 }
 
-template <typename T, int VB, int U>
-__global__ void __launch_bounds__(256) qk_vec_forward_kernel(const QkVec v) {
+// The token and heads of an item.
+struct Item { int pos, h0, h1; const unsigned char* x; unsigned char* y; unsigned char* dx; };
+template <bool BACKWARD> __device__ __forceinline__ Item item_of(const QkVec& v, const QkSide& sd, uint32_t i) {
+    Item m{};
+    m.pos = -1;
+    if (i >= sd.items) return m;
+    const uint32_t t = div_by(i, sd.chunks_mul, sd.chunks_shift), chunk = i - t * sd.chunks;
+    const uint32_t b = div_by(t, v.l_mul, v.l_shift), l = t - b * v.L;
+    m.h0 = static_cast<int>(chunk) * sd.per_item;
+    m.h1 = min(m.h0 + sd.per_item, sd.H);
+    m.pos = v.positions ? v.positions[static_cast<long long>(b) * v.pos_b + l] : static_cast<int>(l);
+    auto at = [&](const QkView& w) {
+        return w.p + static_cast<uint64_t>(b) * w.b + static_cast<uint64_t>(l) * w.l + static_cast<uint64_t>(static_cast<uint32_t>(m.h0)) * w.h;
+    };
+    m.x = at(sd.x); m.y = at(sd.y);
+    if (BACKWARD) m.dx = at(sd.dx);
+    return m;
+}
+
+template <typename T, int VB, int U, int BLOCKS>
+__global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const QkVec v) {
     constexpr int V = VB / sizeof(T);
     using Raw = typename RawOf<VB>::type;
+    __shared__ float weights[kQkMaxDim + 32];      // a lane past the end of a row reads behind it
     pdl_wait();
     pdl_launch_dependents();
-    const bool key = blockIdx.x >= v.blocks_q;
-    const Side sd = side_of(v, key);
-    const QkStep& st = key ? v.step_k : v.step_q;
-    const int lane = threadIdx.x & 31, l = lane & (v.G - 1), g = lane / v.G;
-    const Lane<V> n = lane_of<V>(v, l);
-    const uint32_t tokens = static_cast<uint32_t>(v.p.B) * static_cast<uint32_t>(v.p.L);
-    const float inv_d = 1.0f / static_cast<float>(v.p.d);
-    float w[2 * V];
+    const bool key = blockIdx.x >= v.side[0].blocks;
+    const QkSide& sd = v.side[key];
+    const int lane = threadIdx.x & 31, W = 32 / v.G;
+    const Lane n = lane_of<V>(v, lane & (v.G - 1));
+    const float inv_d = 1.0f / static_cast<float>(v.d);
+    const uint32_t warp = (blockIdx.x - (key ? v.side[0].blocks : 0u)) * 8u + (threadIdx.x >> 5), step = sd.blocks * 8u * W;
+    for (int e = threadIdx.x; e < kQkMaxDim + 32; e += 256) weights[e] = sd.w && e < v.d ? sd.w[e] : 1.0f;
+    __syncthreads();
+    for (uint32_t first = warp * W; first < sd.items; first += step) {
+        Item m = item_of<false>(v, sd, first + lane / v.G);
+        // the result is rs * (x_a (w_a c) - x_b (w_b s), x_b (w_b c) + x_a (w_a s))
+        float ac[V], bs[V], bc[V], as[V];
+        load_table<V>(v, n, max(m.pos, 0), bc, as);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        w[i] = sd.w && n.has_a ? sd.w[n.a + i] : 1.0f;
-        w[V + i] = sd.w && n.has_b ? sd.w[n.b + i] : 1.0f;
-    }
-    const long long warp = (blockIdx.x - (key ? v.blocks_q : 0u)) * 8ll + (threadIdx.x >> 5);
-    const long long r0 = warp * (U * (32 / v.G)) + g;
-    At first{static_cast<uint32_t>(min(r0 / sd.H, 0x7fffffffll)), static_cast<int>(r0 % sd.H)};
-    for (long long batch = warp; batch < st.batches; batch += st.warps) {
-        Raw ra[U], rb[U];
-        uint32_t b[U], pl[U]; int h[U], pos[U];
-        At r = first;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = r.t < tokens;
-            const uint32_t t = in ? r.t : 0u;
-            b[u] = div_by(t, v.l_mul, v.l_shift); pl[u] = t - b[u] * static_cast<uint32_t>(v.p.L); h[u] = r.h;
-            pos[u] = !in ? -1 : v.p.positions ? v.p.positions[b[u] * v.p.pos_b + pl[u]] : static_cast<int>(pl[u]);
-            const T* src = static_cast<const T*>(sd.x.p) + b[u] * sd.x.b + pl[u] * sd.x.l + h[u] * sd.x.h;
-            ra[u] = Raw{}; rb[u] = Raw{};
-            if (in && n.has_a) ra[u] = *reinterpret_cast<const Raw*>(src + n.a);
-            if (in && n.has_b) rb[u] = *reinterpret_cast<const Raw*>(src + n.b);
-            advance(r, st.sub_t, st.sub_h, sd.H);
+        for (int i = 0; i < V; ++i) {              // neighbours: the lane's two chunks are one run of V pairs
+            const float wa = v.interleaved ? weights[n.a + 2 * i] : weights[n.a + i], wb = v.interleaved ? weights[n.a + 2 * i + 1] : weights[n.b + i];
+            ac[i] = wa * bc[i]; bs[i] = -wb * as[i]; bc[i] = wb * bc[i]; as[i] = wa * as[i];
         }
+        const bool padding = m.pos < 0;
+        const int count = m.h1 - m.h0;
+        for (int h = 0; h < sd.per_item; h += U) {
+            Raw ra[U], rb[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float x[2 * V], c[V], s[V];
-            load_table<V>(v, n, pos[u] < 0 ? 0 : pos[u], c, s);
-            unpack<T, VB>(ra[u], x);
-            unpack<T, VB>(rb[u], x + V);
-            if (v.p.norm == 2) {
-                float m = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) m += x[i];
-                m = group_sum(m, v.G) * inv_d;
-#pragma unroll
-                for (int i = 0; i < V; ++i) { x[i] = n.has_a ? x[i] - m : 0.0f; x[V + i] = n.has_b ? x[V + i] - m : 0.0f; }
+            for (int u = 0; u < U; ++u) {
+                ra[u] = Raw{}; rb[u] = Raw{};
+                const T* src = reinterpret_cast<const T*>(m.x + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.x.h);
+                if (h + u < count && n.has_a) ra[u] = *reinterpret_cast<const Raw*>(src + n.a);
+                if (h + u < count && n.has_b) rb[u] = *reinterpret_cast<const Raw*>(src + n.b);
             }
-            float rs = 1.0f;
-            if (v.p.norm != 0) {
-                float q = 0.0f;
+            m.x += static_cast<uint64_t>(U) * sd.x.h;
 #pragma unroll
-                for (int i = 0; i < 2 * V; ++i) q = fmaf(x[i], x[i], q);
-                rs = 1.0f / sqrtf(fmaf(group_sum(q, v.G), inv_d, v.p.eps));
-            }
+            for (int u = 0; u < U; ++u) {
+                float x[2 * V], y[2 * V];
+                unpack<T, VB>(ra[u], x);
+                unpack<T, VB>(rb[u], x + V);
+                const float rs = normalizer<V>(v, n, inv_d, x);
+                if (v.interleaved) {
 #pragma unroll
-            for (int i = 0; i < 2 * V; ++i) x[i] = x[i] * rs * w[i];
-            turn<V, 1>(x, c, s, v.p, n);
-            if (pos[u] >= 0) {
-                T* dst = static_cast<T*>(sd.y.p) + b[u] * sd.y.b + pl[u] * sd.y.l + h[u] * sd.y.h;
-                if (n.has_a) *reinterpret_cast<Raw*>(dst + n.a) = pack<T, VB>(x);
-                if (n.has_b) *reinterpret_cast<Raw*>(dst + n.b) = pack<T, VB>(x + V);
+                    for (int i = 0; i < V; ++i) {
+                        const float a = x[2 * i] * rs, b = x[2 * i + 1] * rs;
+                        y[2 * i] = fmaf(b, bs[i], a * ac[i]);
+                        y[2 * i + 1] = fmaf(a, as[i], b * bc[i]);
+                    }
+                } else if constexpr (V % 2 == 0) {
+                    const uint64_t r2 = pack2(rs, rs);
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) {
+                        const uint64_t a = fmul2(pack2(x[i], x[i + 1]), r2), b = fmul2(pack2(x[V + i], x[V + i + 1]), r2);
+                        unpack2(ffma2(b, pack2(bs[i], bs[i + 1]), fmul2(a, pack2(ac[i], ac[i + 1]))), y[i], y[i + 1]);
+                        unpack2(ffma2(a, pack2(as[i], as[i + 1]), fmul2(b, pack2(bc[i], bc[i + 1]))), y[V + i], y[V + i + 1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float a = x[i] * rs, b = x[V + i] * rs;
+                        y[i] = fmaf(b, bs[i], a * ac[i]);
+                        y[V + i] = fmaf(a, as[i], b * bc[i]);
+                    }
+                }
+                if (!v.all_turn) {                 // dims that pass: an infinity must not meet a neighbour, not even times 0
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        if (n.turns && n.pair + i < v.rot / 2) continue;
+                        if (v.interleaved) { y[2 * i] = x[2 * i] * rs * ac[i]; y[2 * i + 1] = x[2 * i + 1] * rs * bc[i]; }
+                        else { y[i] = x[i] * rs * ac[i]; y[V + i] = x[V + i] * rs * bc[i]; }
+                    }
+                }
+                if (h + u < count && !padding) {
+                    T* dst = reinterpret_cast<T*>(m.y + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.y.h);
+                    if (n.has_a) *reinterpret_cast<Raw*>(dst + n.a) = pack<T, VB>(y);
+                    if (n.has_b) *reinterpret_cast<Raw*>(dst + n.b) = pack<T, VB>(y + V);
+                }
             }
+            m.y += static_cast<uint64_t>(U) * sd.y.h;
         }
-        advance(first, st.jump_t, st.jump_h, sd.H);
     }
 }
 
-template <typename T, int VB, int U>
-__global__ void __launch_bounds__(256) qk_vec_backward_kernel(const QkVec v) {
+template <typename T, int VB, int U, int BLOCKS>
+__global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const QkVec v) {
     constexpr int V = VB / sizeof(T);
     using Raw = typename RawOf<VB>::type;
     extern __shared__ float sums[];                // [8][d]
+    __shared__ float weights[kQkMaxDim + 32];
     pdl_wait();
     pdl_launch_dependents();
-    const bool key = blockIdx.x >= v.blocks_q;
-    const Side sd = side_of(v, key);
-    const QkStep& st = key ? v.step_k : v.step_q;
-    const int lane = threadIdx.x & 31, l = lane & (v.G - 1), g = lane / v.G;
-    const Lane<V> n = lane_of<V>(v, l);
-    const uint32_t tokens = static_cast<uint32_t>(v.p.B) * static_cast<uint32_t>(v.p.L);
-    const float inv_d = 1.0f / static_cast<float>(v.p.d);
-    float w[2 * V], dw[2 * V];
+    const bool key = blockIdx.x >= v.side[0].blocks;
+    const QkSide& sd = v.side[key];
+    const int lane = threadIdx.x & 31, W = 32 / v.G;
+    const Lane n = lane_of<V>(v, lane & (v.G - 1));
+    const float inv_d = 1.0f / static_cast<float>(v.d);
+    const uint32_t warp = (blockIdx.x - (key ? v.side[0].blocks : 0u)) * 8u + (threadIdx.x >> 5), step = sd.blocks * 8u * W;
+    for (int e = threadIdx.x; e < kQkMaxDim + 32; e += 256) weights[e] = sd.w && e < v.d ? sd.w[e] : 1.0f;
+    __syncthreads();
+    float dw[2 * V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        w[i] = sd.w && n.has_a ? sd.w[n.a + i] : 1.0f;
-        w[V + i] = sd.w && n.has_b ? sd.w[n.b + i] : 1.0f;
-        dw[i] = dw[V + i] = 0.0f;
-    }
-    const long long warp = (blockIdx.x - (key ? v.blocks_q : 0u)) * 8ll + (threadIdx.x >> 5);
-    const long long r0 = warp * (U * (32 / v.G)) + g;
-    At first{static_cast<uint32_t>(min(r0 / sd.H, 0x7fffffffll)), static_cast<int>(r0 % sd.H)};
-    for (long long batch = warp; batch < st.batches; batch += st.warps) {
-        Raw ra[U], rb[U], ga[U], gb[U];
-        uint32_t b[U], pl[U]; int h[U], pos[U]; bool in[U];
-        At r = first;
+    for (int i = 0; i < 2 * V; ++i) dw[i] = 0.0f;
+    for (uint32_t first = warp * W; first < sd.items; first += step) {
+        Item m = item_of<true>(v, sd, first + lane / v.G);
+        float c[V], s[V];
+        load_table<V>(v, n, max(m.pos, 0), c, s);
+        const bool padding = m.pos < 0;
+        const int count = m.h1 - m.h0;
+        for (int h = 0; h < sd.per_item; h += U) {
+            Raw ra[U], rb[U], ga[U], gb[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            in[u] = r.t < tokens;
-            const uint32_t t = in[u] ? r.t : 0u;
-            b[u] = div_by(t, v.l_mul, v.l_shift); pl[u] = t - b[u] * static_cast<uint32_t>(v.p.L); h[u] = r.h;
-            pos[u] = !in[u] ? -1 : v.p.positions ? v.p.positions[b[u] * v.p.pos_b + pl[u]] : static_cast<int>(pl[u]);
-            const T* src = static_cast<const T*>(sd.x.p) + b[u] * sd.x.b + pl[u] * sd.x.l + h[u] * sd.x.h;
-            const T* dy = static_cast<const T*>(sd.y.p) + b[u] * sd.y.b + pl[u] * sd.y.l + h[u] * sd.y.h;
-            ra[u] = rb[u] = ga[u] = gb[u] = Raw{};
-            if (in[u] && n.has_a) { ra[u] = *reinterpret_cast<const Raw*>(src + n.a); ga[u] = *reinterpret_cast<const Raw*>(dy + n.a); }
-            if (in[u] && n.has_b) { rb[u] = *reinterpret_cast<const Raw*>(src + n.b); gb[u] = *reinterpret_cast<const Raw*>(dy + n.b); }
-            advance(r, st.sub_t, st.sub_h, sd.H);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float x[2 * V], y[2 * V], c[V], s[V];
-            load_table<V>(v, n, pos[u] < 0 ? 0 : pos[u], c, s);
-            if (pos[u] < 0) ra[u] = rb[u] = ga[u] = gb[u] = Raw{};             // padding may hold anything: its gradients are 0
-            unpack<T, VB>(ra[u], x);
-            unpack<T, VB>(rb[u], x + V);
-            unpack<T, VB>(ga[u], y);
-            unpack<T, VB>(gb[u], y + V);
-            turn<V, -1>(y, c, s, v.p, n);
-            if (v.p.norm == 2) {
-                float m = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 2 * V; ++i) m += x[i];
-                m = group_sum(m, v.G) * inv_d;
-#pragma unroll
-                for (int i = 0; i < V; ++i) { x[i] = n.has_a ? x[i] - m : 0.0f; x[V + i] = n.has_b ? x[V + i] - m : 0.0f; }
+            for (int u = 0; u < U; ++u) {
+                ra[u] = rb[u] = ga[u] = gb[u] = Raw{};
+                if (h + u >= count || padding) continue;       // padding may hold anything: its gradients are 0
+                const T* src = reinterpret_cast<const T*>(m.x + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.x.h);
+                const T* dy = reinterpret_cast<const T*>(m.y + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.y.h);
+                if (n.has_a) { ra[u] = *reinterpret_cast<const Raw*>(src + n.a); ga[u] = *reinterpret_cast<const Raw*>(dy + n.a); }
+                if (n.has_b) { rb[u] = *reinterpret_cast<const Raw*>(src + n.b); gb[u] = *reinterpret_cast<const Raw*>(dy + n.b); }
             }
-            float rs = 1.0f;
-            if (v.p.norm != 0) {
-                float q = 0.0f;
+            m.x += static_cast<uint64_t>(U) * sd.x.h;
+            m.y += static_cast<uint64_t>(U) * sd.y.h;
 #pragma unroll
-                for (int i = 0; i < 2 * V; ++i) q = fmaf(x[i], x[i], q);
-                rs = 1.0f / sqrtf(fmaf(group_sum(q, v.G), inv_d, v.p.eps));
-            }
-            float sg = 0.0f, sgx = 0.0f;
+            for (int u = 0; u < U; ++u) {
+                float x[2 * V], y[2 * V];
+                unpack<T, VB>(ra[u], x);
+                unpack<T, VB>(rb[u], x + V);
+                unpack<T, VB>(ga[u], y);
+                unpack<T, VB>(gb[u], y + V);
+                if (n.turns) {
+                    if (v.interleaved) {
 #pragma unroll
-            for (int i = 0; i < 2 * V; ++i) {
-                x[i] *= rs;
-                if (pos[u] >= 0) dw[i] = fmaf(y[i], x[i], dw[i]);              // eps = 0 makes a padded row's xhat NaN
-                y[i] *= w[i];
-                sg += y[i];
-                sgx = fmaf(y[i], x[i], sgx);
-            }
-            if (v.p.norm != 0) {
-                sgx = group_sum(sgx, v.G) * inv_d;
-                sg = v.p.norm == 2 ? group_sum(sg, v.G) * inv_d : 0.0f;
+                        for (int i = 0; i < V; ++i) {
+                            if (!v.all_turn && n.pair + i >= v.rot / 2) continue;
+                            const float a = y[2 * i], b = y[2 * i + 1];
+                            y[2 * i] = fmaf(b, s[i], a * c[i]);
+                            y[2 * i + 1] = fmaf(-a, s[i], b * c[i]);
+                        }
+                    } else {
 #pragma unroll
-                for (int i = 0; i < 2 * V; ++i) y[i] = rs * (y[i] - sg - x[i] * sgx);
-            }
-            if (in[u]) {
-                if (pos[u] < 0) {
-#pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) y[i] = 0.0f;
+                        for (int i = 0; i < V; ++i) {
+                            const float a = y[i], b = y[V + i];
+                            y[i] = fmaf(b, s[i], a * c[i]);
+                            y[V + i] = fmaf(-a, s[i], b * c[i]);
+                        }
+                    }
                 }
-                T* dst = static_cast<T*>(sd.dx.p) + b[u] * sd.dx.b + pl[u] * sd.dx.l + h[u] * sd.dx.h;
-                if (n.has_a) *reinterpret_cast<Raw*>(dst + n.a) = pack<T, VB>(y);
-                if (n.has_b) *reinterpret_cast<Raw*>(dst + n.b) = pack<T, VB>(y + V);
+                __syncwarp();
+                const bool live = h + u < count && !padding;
+                const float rs = normalizer<V>(v, n, inv_d, x);
+#pragma unroll
+                for (int i = 0; i < 2 * V; ++i) {
+                    x[i] *= rs;
+                    if (live) dw[i] = fmaf(y[i], x[i], dw[i]); // eps = 0 makes the xhat of a row of zeros NaN
+                    y[i] *= weights[i < V ? n.a + i : n.b + i - V];
+                }
+                if (v.norm != 0) {
+                    const float sgx = group_sum(lane_dot(y, x), v.G) * inv_d;
+                    const float sg = v.norm == 2 ? group_sum(lane_sum(y), v.G) * inv_d : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 2 * V; ++i) y[i] = rs * (fmaf(-x[i], sgx, y[i]) - sg);
+                }
+                if (h + u < count) {
+                    if (padding) {
+#pragma unroll
+                        for (int i = 0; i < 2 * V; ++i) y[i] = 0.0f;
+                    }
+                    T* dst = reinterpret_cast<T*>(m.dx + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.dx.h);
+                    if (n.has_a) *reinterpret_cast<Raw*>(dst + n.a) = pack<T, VB>(y);
+                    if (n.has_b) *reinterpret_cast<Raw*>(dst + n.b) = pack<T, VB>(y + V);
+                }
             }
+            m.dx += static_cast<uint64_t>(U) * sd.dx.h;
         }
-        advance(first, st.jump_t, st.jump_h, sd.H);
     }
-    if (!v.p.partial) return;
+    if (!v.partial) return;
     // the rows of a warp, then the warps of the block in order: one line of the workspace per block
 #pragma unroll
     for (int i = 0; i < 2 * V; ++i)
         for (int o = v.G; o < 32; o <<= 1) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-    float* mine = sums + (threadIdx.x >> 5) * v.p.d;
-    if (g == 0) {
+    float* mine = sums + (threadIdx.x >> 5) * v.d;
+    if (lane < v.G) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (n.has_a) mine[n.a + i] = dw[i];
@@ -495,11 +529,11 @@ __global__ void __launch_bounds__(256) qk_vec_backward_kernel(const QkVec v) {
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < v.p.d; e += 256) {
-        float s = 0.0f;
+    for (int e = threadIdx.x; e < v.d; e += 256) {
+        float t = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) s += sums[k * v.p.d + e];
-        v.p.partial[static_cast<long long>(blockIdx.x) * v.p.d + e] = s;
+        for (int k = 0; k < 8; ++k) t += sums[k * v.d + e];
+        v.partial[static_cast<long long>(blockIdx.x) * v.d + e] = t;
     }
 }
 
@@ -530,58 +564,76 @@ unsigned blocks_for(long long rows, int per_block) {
     return static_cast<unsigned>(b < kQkMaxBlocks ? b : kQkMaxBlocks);
 }
 
-QkStep step_for(long long rows, int H, int per_warp, int W, unsigned blocks) {
-    QkStep s{};
-    s.batches = (rows + per_warp - 1) / per_warp;
-    s.warps = 8ll * blocks;
-    const long long jump = s.warps * per_warp;
-    s.jump_t = H ? static_cast<uint32_t>(jump / H) : 0; s.jump_h = H ? static_cast<int>(jump % H) : 0;
-    s.sub_t = H ? W / H : 0; s.sub_h = H ? W % H : 0;
-    return s;
+void divisor(uint32_t d, uint32_t* mul, int* shift) {
+    *mul = 0; *shift = 0;
+    if (d <= 1) return;
+    while (*shift < 30 && (2u << *shift) < d) ++*shift;
+    *mul = static_cast<uint32_t>(((1ull << (32 + *shift)) + d - 1) / d);
 }
 
-template <typename T, int VB, int U>
-cudaError_t launch_vec(QkVec& v, bool backward, cudaStream_t st) {
+template <typename T, int VB>
+cudaError_t launch_vec(const QkParams& p, QkVec& v, bool backward, cudaStream_t st) {
     constexpr int V = VB / sizeof(T);
-    const int chunks = v.p.d / V, half = v.p.interleaved ? 0 : v.p.rot / 2 / V;
+    const int chunks = p.d / V, half = p.interleaved ? 0 : p.rot / 2 / V;
     const int pairs = half + (chunks - 2 * half + 1) / 2;
     v.G = 1;
     while (v.G < pairs) v.G *= 2;
-    const int W = 32 / v.G, per_warp = U * W;
-    const long long tokens = static_cast<long long>(v.p.B) * v.p.L, rq = tokens * v.p.hq, rk = tokens * v.p.hk;
-    // forward: eight batches a warp at most keep the last wave short; backward: few blocks, as each leaves a line to be summed
-    const long long cap = backward ? 2ll * num_sms() : 16ll * num_sms();
-    long long bq = (rq + 8 * per_warp - 1) / (8 * per_warp), bk = (rk + 8 * per_warp - 1) / (8 * per_warp);
-    if (bq + bk > cap) {
-        const long long all = bq + bk;
-        bq = bq ? std::max(1ll, cap * bq / all) : 0;
-        bk = bk ? std::max(1ll, cap - bq) : 0;
+    v.all_turn = p.rot == p.d;
+    v.table_vec = (reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t)) % 16 == 0 && (p.rot / 2) % 4 == 0 &&
+                  (!p.interleaved || (p.rot / 2) % V == 0);
+    const int W = 32 / v.G, sms = num_sms();
+    const long long tokens = static_cast<long long>(p.B) * p.L;
+    // an item per token where that gives every SM 64 warps or more of them (a few rounds of what is resident), else the heads in
+    // several items, of as many heads as are loaded at once
+    const long long wanted = 64ll * sms * W;
+    long long warps[2];
+    for (int k = 0; k < 2; ++k) {
+        QkSide& sd = v.side[k];
+        const int H = k ? p.hk : p.hq;
+        const long long cuts = std::min<long long>(std::max(H, 1), std::max(1ll, wanted / tokens));
+        sd.H = H;
+        sd.per_item = std::max(1, static_cast<int>((H + cuts - 1) / cuts));
+        sd.per_item = std::min(std::max(H, 1), (sd.per_item + kHeadsAtOnce - 1) / kHeadsAtOnce * kHeadsAtOnce);
+        sd.chunks = std::max(1, (H + sd.per_item - 1) / sd.per_item);
+        sd.items = H ? static_cast<uint32_t>(tokens * sd.chunks) : 0u;
+        divisor(static_cast<uint32_t>(sd.chunks), &sd.chunks_mul, &sd.chunks_shift);
+        warps[k] = (static_cast<long long>(sd.items) + W - 1) / W;
     }
-    v.blocks_q = static_cast<unsigned>(bq);
-    v.step_q = step_for(rq, v.p.hq, per_warp, W, v.blocks_q);
-    v.step_k = step_for(rk, v.p.hk, per_warp, W, static_cast<unsigned>(bk));
+    // forward: blocks to fill the SMs eight times over; backward: few, as each leaves a line of weight gradients to be summed
+    const long long cap = (backward ? 2ll : 8ll) * sms;
+    long long bq = (warps[0] + 7) / 8, bk = (warps[1] + 7) / 8;
+    if (bq + bk > cap) {                           // in proportion to the rows
+        const long long share = cap * p.hq / (p.hq + p.hk);
+        bq = bq ? std::min(bq, std::max(1ll, share)) : 0;
+        bk = bk ? std::min(bk, std::max(1ll, cap - bq)) : 0;
+    }
+    v.side[0].blocks = static_cast<uint32_t>(bq); v.side[1].blocks = static_cast<uint32_t>(bk);
     const dim3 grid(static_cast<unsigned>(bq + bk));
-    if (!backward) return launch_pdl(qk_vec_forward_kernel<T, VB, U>, grid, dim3(256), 0, st, v);
-    cudaError_t e = launch_pdl(qk_vec_backward_kernel<T, VB, U>, grid, dim3(256), v.p.partial ? 8u * v.p.d * sizeof(float) : 0u, st, v);
-    if (e == cudaSuccess && v.p.partial)
-        e = launch_pdl(qk_weight_sum_kernel, dim3((v.p.d + 31) / 32, 2), dim3(1024), 0, st, static_cast<const float*>(v.p.partial), static_cast<int>(bq),
-                       static_cast<int>(bk), v.p.d, v.p.dqw, v.p.dkw);
+    if (!backward) return launch_pdl(qk_vec_forward_kernel<T, VB, kHeadsAtOnce, V == 8 ? 2 : V == 4 ? 3 : 4>, grid, dim3(256), 0, st, v);
+    cudaError_t e = launch_pdl(qk_vec_backward_kernel<T, VB, V == 8 ? 2 : 4, 2>, grid, dim3(256), v.partial ? 8u * p.d * sizeof(float) : 0u, st, v);
+    if (e == cudaSuccess && v.partial)
+        e = launch_pdl(qk_weight_sum_kernel, dim3((p.d + 31) / 32, 2), dim3(1024), 0, st, static_cast<const float*>(v.partial), static_cast<int>(bq),
+                       static_cast<int>(bk), p.d, p.dqw, p.dkw);
     return e;
 }
 
-// The widest chunk that every base, stride and boundary of the call allows: 16, 8 or 4 bytes, 0 for none.
+// The widest chunk that every base, stride and boundary of the call allows: 16, 8 or 4 bytes; 0 for none, or for strides beyond 32 bits.
 int chunk_bytes(const QkParams& p, bool backward, int elem) {
-    uintptr_t bits = static_cast<uintptr_t>(p.d) * elem;
-    if (p.rot > 0 && !p.interleaved) bits |= static_cast<uintptr_t>(p.rot / 2) * elem;
+    uint64_t bits = static_cast<uint64_t>(p.d) * elem, most = 0;
+    if (p.rot > 0 && !p.interleaved) bits |= static_cast<uint64_t>(p.rot / 2) * elem;
+    auto stride = [&](long long s, int extent) {
+        if (extent <= 1) return;
+        most = std::max(most, static_cast<uint64_t>(s));
+        bits |= static_cast<uint64_t>(s) * elem;
+    };
     auto add = [&](const HeadsView& h, int heads) {
         if (heads == 0) return;
         bits |= reinterpret_cast<uintptr_t>(h.p);
-        if (p.B > 1) bits |= static_cast<uintptr_t>(h.b) * elem;
-        if (p.L > 1) bits |= static_cast<uintptr_t>(h.l) * elem;
-        if (heads > 1) bits |= static_cast<uintptr_t>(h.h) * elem;
+        stride(h.b, p.B); stride(h.l, p.L); stride(h.h, heads);
     };
     add(p.q, p.hq); add(p.k, p.hk); add(p.qo, p.hq); add(p.ko, p.hk);
     if (backward) { add(p.dq, p.hq); add(p.dk, p.hk); }
+    if (most > UINT32_MAX / 4) return 0;
     for (int vb = 16; vb >= 4; vb /= 2)
         if (bits % vb == 0 && vb >= elem) return p.d * elem <= 64 * vb ? vb : 0;
     return 0;
@@ -589,20 +641,24 @@ int chunk_bytes(const QkParams& p, bool backward, int elem) {
 
 template <typename T>
 int launch_any(const QkParams& p, bool backward, cudaStream_t st) {
-    QkVec v{};
-    v.p = p;
     const int vb = chunk_bytes(p, backward, sizeof(T));
     cudaError_t e;
     if (vb) {
-        const uint32_t L = static_cast<uint32_t>(p.L);
-        if (L > 1) {
-            while ((2u << v.l_shift) < L && v.l_shift < 30) ++v.l_shift;
-            v.l_mul = static_cast<uint32_t>(((1ull << (32 + v.l_shift)) + L - 1) / L);
+        QkVec v{};
+        auto view = [&](const HeadsView& h, int heads) {       // a stride of an extent of 1 is never used
+            auto bytes = [](long long s, int n) { return n > 1 ? static_cast<uint32_t>(s * sizeof(T)) : 0u; };
+            return QkView{static_cast<unsigned char*>(h.p), bytes(h.b, p.B), bytes(h.l, p.L), bytes(h.h, heads)};
+        };
+        for (int k = 0; k < 2; ++k) {
+            const int H = k ? p.hk : p.hq;
+            v.side[k].x = view(k ? p.k : p.q, H); v.side[k].y = view(k ? p.ko : p.qo, H); v.side[k].dx = view(k ? p.dk : p.dq, H);
+            v.side[k].w = k ? p.kw : p.qw;
         }
-        v.table_vec = (reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t)) % 16 == 0 && (p.rot / 2) % 4 == 0 &&
-                      (!p.interleaved || (p.rot / 2) % (vb / sizeof(T)) == 0);
-        e = vb == 16 ? launch_vec<T, 16, sizeof(T) == 4 ? 4 : 2>(v, backward, st)
-                     : vb == 8 ? launch_vec<T, 8, 4>(v, backward, st) : launch_vec<T, 4, 4>(v, backward, st);
+        v.cos_t = p.cos_t; v.sin_t = p.sin_t; v.positions = p.positions; v.partial = p.partial; v.pos_b = p.pos_b;
+        v.L = static_cast<uint32_t>(p.L); v.d = p.d; v.rot = p.rot; v.norm = p.norm; v.interleaved = p.interleaved; v.table_rows = p.table_rows;
+        v.eps = p.eps;
+        divisor(v.L, &v.l_mul, &v.l_shift);
+        e = vb == 16 ? launch_vec<T, 16>(p, v, backward, st) : vb == 8 ? launch_vec<T, 8>(p, v, backward, st) : launch_vec<T, 4>(p, v, backward, st);
     } else {
         const unsigned grid = blocks_for(static_cast<long long>(p.B) * p.L * (p.hq + p.hk), kWarps);
         const int n = (p.d + 31) / 32;
