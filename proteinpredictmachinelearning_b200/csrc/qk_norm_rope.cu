@@ -28,7 +28,8 @@ struct QkVec {
     const float* cos_t; const float* sin_t; const int* positions; float* partial;
     long long pos_b;
     uint32_t L, l_mul; int l_shift;                // division by L
-    int d, rot, norm, interleaved, table_rows, table_vec, all_turn;
+    int d, rot, norm, interleaved, table_rows, table_vec;
+    int all_turn, full;                            // every value turns; every lane holds 2 V values
     int G;                                         // lanes per row
     float eps;
 };
@@ -219,30 +220,49 @@ __global__ void __launch_bounds__(32 * kWarps) qk_backward_kernel(const QkParams
 // ---- vector kernels ----------------------------------------------------------------------------------------------------
 // A lane holds two chunks of V neighbouring values (VB bytes each) that rotate with one another: chunks l and l + rot / 2 / V for
 // the pairs (i, i + rot / 2), chunks 2 l and 2 l + 1 for neighbouring pairs and for dims that pass.  So a rotation needs no
-// exchange between lanes.  G lanes (a power of two) hold a row, a warp 32 / G of them, of different tokens: each group of
-// lanes walks over the heads of its token, so that the position, its table row, the weights and all but one addition of
-// an address are had once per token instead of once per row (20 instructions a value before, 6 now).  A block works on one
-// side (Q or K).  Where there are few tokens the heads are dealt to several items.
-constexpr int kHeadsAtOnce = 4;                    // rows per lane whose loads are in flight together (forward)
+// exchange between lanes, and two values go by one packed instruction.  G lanes (a power of two) hold a row, a warp 32 / G of
+// them, of different tokens: each group of lanes walks over the heads of its token, so that the position, its table row and
+// all but one addition of an address are had once per token instead of once per row.  A block works on one side (Q or K).
+// What bounds it: the bytes in flight.  Rows wait in registers from the load to the store, and 16 (bf16) to 24 (fp32) warps an SM are
+// what that leaves; a ring of rows in shared memory (cp.async) kept more in flight and cost 40 instructions a row: 120 against
+// 122 us on the long case below, 43 against 34 on the short one, and was dropped.
+// Measured (forward): 65536 tokens x 16 heads of 32, fp32 45 us (5.9 TB/s); 32768 tokens x 40 heads of 128, bf16 124 us (5.4 TB/s);
+// 16384 tokens x 32 heads of 64, bf16, LayerNorm, neighbouring pairs 35 us; backward of the last 54 us (3.8 TB/s), of 16384 tokens x 16
+// heads of 32, fp32 25 us.
+constexpr int kHeadsAtOnce = 4;                    // rows of a group of lanes that are loaded together (forward)
 
 template <int VB> struct RawOf;
 template <> struct RawOf<16> { using type = uint4; };
 template <> struct RawOf<8> { using type = uint2; };
 template <> struct RawOf<4> { using type = uint32_t; };
 
-template <typename T, int VB> __device__ __forceinline__ void unpack(const typename RawOf<VB>::type& raw, float* x) {
-    constexpr int V = VB / sizeof(T);
-    const T* t = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = to_f32(t[i]);
+// The lane's 2 V values as V packed pairs: pair j holds values 2 j and 2 j + 1 of its two chunks one behind the other (V = 1: one of
+// each).  All arithmetic goes by packed instructions.
+template <typename T> __device__ __forceinline__ uint64_t widen(uint32_t two) {
+    if constexpr (sizeof(T) == 2) {
+        const uint16_t lo = static_cast<uint16_t>(two & 0xffffu), hi = static_cast<uint16_t>(two >> 16);
+        return pack2(to_f32(*reinterpret_cast<const T*>(&lo)), to_f32(*reinterpret_cast<const T*>(&hi)));
+    }
+    return 0;
 }
-template <typename T, int VB> __device__ __forceinline__ typename RawOf<VB>::type pack(const float* x) {
-    constexpr int V = VB / sizeof(T);
-    typename RawOf<VB>::type raw;
-    T* t = reinterpret_cast<T*>(&raw);
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __nv_bfloat16) { const __nv_bfloat162 t = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __half) { const __half2 t = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
+__device__ __forceinline__ uint32_t narrow2(float a, float, float) { return __float_as_uint(a); }
+template <typename T, int VB> __device__ __forceinline__ void store_pairs(const uint64_t (&y)[VB / sizeof(T)], unsigned char* to, uint32_t a, uint32_t b, bool has_a, bool has_b) {
+    constexpr int V = VB / sizeof(T), kWords = VB / 4;
+    uint32_t w[2 * kWords];
 #pragma unroll
-    for (int i = 0; i < V; ++i) t[i] = from_f32<T>(x[i]);
-    return raw;
+    for (int j = 0; j < V; ++j) {
+        float lo, hi;
+        unpack2(y[j], lo, hi);
+        if constexpr (sizeof(T) == 2) w[j] = narrow2(lo, hi, T());
+        else { w[2 * j] = __float_as_uint(lo); w[2 * j + 1] = __float_as_uint(hi); }
+    }
+    typename RawOf<VB>::type ra, rb;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) { reinterpret_cast<uint32_t*>(&ra)[i] = w[i]; reinterpret_cast<uint32_t*>(&rb)[i] = w[kWords + i]; }
+    if (has_a) *reinterpret_cast<typename RawOf<VB>::type*>(to + a) = ra;
+    if (has_b) *reinterpret_cast<typename RawOf<VB>::type*>(to + b) = rb;
 }
 
 // n / d for n < 2^31: with 2^s < d <= 2^(s + 1) and m = ceil(2^(32 + s) / d) the error m d - 2^(32 + s) is below 2^(s + 1), so that
@@ -256,26 +276,28 @@ __device__ __forceinline__ float inv_sqrt(float v) {
     return r > 0.0f && r < __uint_as_float(0x7f800000u) ? fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r) : r;
 }
 
-// This lane's part of a row and where its pair stands in the table.
-struct Lane { uint32_t a, b; int pair; bool has_a, has_b, turns; };      // a, b: elements
-template <int V> __device__ __forceinline__ Lane lane_of(const QkVec& v, int l) {
+// This lane's part of a row (element and byte offsets of its chunks) and where its pairs stand in the table.
+struct Lane { int a, b, pair, turning; uint32_t at_a, at_b; bool has_a, has_b; };      // turning: packed pairs that turn
+template <typename T, int VB> __device__ __forceinline__ Lane lane_of(const QkVec& v, int l) {
+    constexpr int V = VB / sizeof(T);
     Lane n;
     const int chunks = v.d / V, half = v.interleaved ? 0 : v.rot / 2 / V;
     const bool halves = l < half;
-    n.turns = v.interleaved ? l * V < v.rot / 2 : halves;
     const int a = halves ? l : 2 * half + 2 * (l - half), b = halves ? l + half : a + 1;
     n.has_a = a < chunks; n.has_b = b < chunks;
     n.pair = l * V;
-    n.a = static_cast<uint32_t>(a * V); n.b = static_cast<uint32_t>(b * V);
+    n.turning = v.interleaved ? min(max(v.rot / 2 - n.pair, 0), V) : halves ? V : 0;
+    n.a = a * V; n.b = b * V;
+    n.at_a = static_cast<uint32_t>(a * VB); n.at_b = static_cast<uint32_t>(b * VB);
     return n;
 }
 // cos and sin of the lane's pairs; NaN beyond the table; 1 and 0 where nothing turns
 template <int V> __device__ __forceinline__ void load_table(const QkVec& v, const Lane& n, int pos, float (&c)[V], float (&s)[V]) {
     const int half = v.rot / 2;
-    const float none = n.turns && pos >= v.table_rows ? __uint_as_float(0x7fffffffu) : 1.0f;
+    const float none = pos >= v.table_rows ? __uint_as_float(0x7fffffffu) : 1.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) { c[i] = n.pair + i < half ? none : 1.0f; s[i] = 0.0f; }
-    if (!n.turns || pos >= v.table_rows) return;
+    for (int i = 0; i < V; ++i) { c[i] = i < n.turning ? none : 1.0f; s[i] = 0.0f; }
+    if (n.turning == 0 || pos >= v.table_rows) return;
     const long long at = static_cast<long long>(pos) * half + n.pair;
     if (V % 4 == 0 && v.table_vec) {
 #pragma unroll
@@ -286,38 +308,108 @@ template <int V> __device__ __forceinline__ void load_table(const QkVec& v, cons
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            if (n.pair + i < half) { c[i] = v.cos_t[at + i]; s[i] = v.sin_t[at + i]; }     // neighbours: may end inside the chunk
+            if (i < n.turning) { c[i] = v.cos_t[at + i]; s[i] = v.sin_t[at + i]; }     // neighbours: may end inside the chunk
     }
 }
 __device__ __forceinline__ float group_sum(float v, int G) {
-    for (int o = G >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+        if (o < G) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// Sum over a row, packed pairs of additions inside the lane.
-template <int N> __device__ __forceinline__ float lane_sum(const float (&x)[N]) {
-    if constexpr (N == 2) return x[0] + x[1];
-    uint64_t t = pack2(x[0], x[1]);
+template <int N> __device__ __forceinline__ float lane_sum(const uint64_t (&x)[N]) {
+    uint64_t t = x[0];
 #pragma unroll
-    for (int i = 2; i < N; i += 2) t = fadd2(t, pack2(x[i], x[i + 1]));
+    for (int j = 1; j < N; ++j) t = fadd2(t, x[j]);
     float a, b; unpack2(t, a, b);
     return a + b;
 }
-template <int N> __device__ __forceinline__ float lane_dot(const float (&x)[N], const float (&y)[N]) {
-    uint64_t t = fmul2(pack2(x[0], x[1]), pack2(y[0], y[1]));
+template <int N> __device__ __forceinline__ float lane_dot(const uint64_t (&x)[N], const uint64_t (&y)[N]) {
+    uint64_t t = fmul2(x[0], y[0]);
 #pragma unroll
-    for (int i = 2; i < N; i += 2) t = ffma2(pack2(x[i], x[i + 1]), pack2(y[i], y[i + 1]), t);
+    for (int j = 1; j < N; ++j) t = ffma2(x[j], y[j], t);
     float a, b; unpack2(t, a, b);
     return a + b;
 }
-// (x - mean) and 1 / sqrt(..) of a row; values that do not exist stay 0
-template <int V> __device__ __forceinline__ float normalizer(const QkVec& v, const Lane& n, float inv_d, float (&x)[2 * V]) {
+// x becomes x - mean; returns 1 / sqrt(..) of the row.  Values that do not exist stay 0.
+template <int V> __device__ __forceinline__ float normalizer(const QkVec& v, const Lane& n, float inv_d, uint64_t (&x)[V]) {
     if (v.norm == 0) return 1.0f;
     if (v.norm == 2) {
         const float m = group_sum(lane_sum(x), v.G) * inv_d;
+        const uint64_t m2 = pack2(-m, -m);
 #pragma unroll
-        for (int i = 0; i < V; ++i) { x[i] = n.has_a ? x[i] - m : 0.0f; x[V + i] = n.has_b ? x[V + i] - m : 0.0f; }
+        for (int j = 0; j < V; ++j) x[j] = fadd2(x[j], m2);
+        if (!v.full) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                float lo, hi; unpack2(x[j], lo, hi);
+                x[j] = pack2((V == 1 || 2 * j < V ? n.has_a : n.has_b) ? lo : 0.0f, (2 * j + 1 < V ? n.has_a : n.has_b) ? hi : 0.0f);
+            }
+        }
     }
     return inv_sqrt(fmaf(group_sum(lane_dot(x, x), v.G), inv_d, v.eps));
+}
+__device__ __forceinline__ uint64_t swap2(uint64_t p) { float a, b; unpack2(p, a, b); return pack2(b, a); }
+// y = x * c + partner * s.  The partner of a packed pair is the same place of the other chunk, or with neighbouring pairs (and with
+// V = 1) its own two values exchanged.  Pairs that do not turn are only scaled: an infinity must not meet a neighbour, not even
+// times 0.
+template <int V> __device__ __forceinline__ void turn(const QkVec& v, const Lane& n, const uint64_t (&x)[V], const uint64_t (&c)[V], const uint64_t (&s)[V],
+                                                      uint64_t (&y)[V]) {
+    if (V == 1 || v.interleaved) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            y[j] = fmul2(x[j], c[j]);
+            if (v.all_turn || j < n.turning) y[j] = ffma2(swap2(x[j]), s[j], y[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = fmul2(x[j], c[j]);
+        if (v.all_turn || n.turning) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) y[j] = ffma2(x[(j + V / 2) % V], s[j], y[j]);
+        }
+    }
+}
+// The factors of turn() from the lane's cos and sin and the weights of its values.
+template <int V> __device__ __forceinline__ void factors(const QkVec& v, const Lane& n, int pos, const float* weights, uint64_t (&c)[V], uint64_t (&s)[V]) {
+    float cs[V], sn[V];
+    load_table<V>(v, n, pos, cs, sn);
+    if (V == 1 || v.interleaved) {                 // the lane's values are one run of V pairs (V = 1: one value of each chunk)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float w0 = weights[n.a + 2 * j], w1 = V == 1 ? weights[n.b] : weights[n.a + 2 * j + 1];
+            c[j] = pack2(w0 * cs[j], w1 * cs[j]);
+            s[j] = pack2(-w1 * sn[j], w0 * sn[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const float c0 = cs[2 * j], c1 = cs[2 * j + 1], s0 = sn[2 * j], s1 = sn[2 * j + 1];
+            const float a0 = weights[n.a + 2 * j], a1 = weights[n.a + 2 * j + 1], b0 = weights[n.b + 2 * j], b1 = weights[n.b + 2 * j + 1];
+            c[j] = pack2(a0 * c0, a1 * c1); c[V / 2 + j] = pack2(b0 * c0, b1 * c1);
+            s[j] = pack2(-b0 * s0, -b1 * s1); s[V / 2 + j] = pack2(a0 * s0, a1 * s1);
+        }
+    }
+}
+// Turns a gradient back, in place, from the lane's cos and sin alone (half the registers of factors()).
+template <int V> __device__ __forceinline__ void turn_back(const QkVec& v, const Lane& n, const float (&c)[V], const float (&s)[V], uint64_t (&y)[V]) {
+    if (V == 1 || v.interleaved) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            if (!(v.all_turn || j < n.turning)) continue;
+            float a, b;
+            unpack2(y[j], a, b);
+            y[j] = pack2(fmaf(b, s[j], a * c[j]), fmaf(-a, s[j], b * c[j]));
+        }
+    } else if (v.all_turn || n.turning) {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            const uint64_t c2 = pack2(c[2 * j], c[2 * j + 1]), s2 = pack2(s[2 * j], s[2 * j + 1]), a = y[j], b = y[V / 2 + j];
+            const uint64_t minus = pack2(-s[2 * j], -s[2 * j + 1]);
+            y[j] = ffma2(b, s2, fmul2(a, c2));
+            y[V / 2 + j] = ffma2(a, minus, fmul2(b, c2));
+        }
+    }
 }
 
 // The token and heads of an item.
@@ -339,193 +431,145 @@ template <bool BACKWARD> __device__ __forceinline__ Item item_of(const QkVec& v,
     return m;
 }
 
+// the two chunks of a row as packed pairs
+template <typename T, int VB> __device__ __forceinline__ void pairs_of(const typename RawOf<VB>::type& a, const typename RawOf<VB>::type& b,
+                                                                       uint64_t (&x)[VB / sizeof(T)]) {
+    constexpr int V = VB / sizeof(T), kWords = VB / 4;
+    uint32_t w[2 * kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) { w[i] = reinterpret_cast<const uint32_t*>(&a)[i]; w[kWords + i] = reinterpret_cast<const uint32_t*>(&b)[i]; }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if constexpr (sizeof(T) == 2) x[j] = widen<T>(w[j]);
+        else x[j] = pack2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+    }
+}
+template <int VB> __device__ __forceinline__ typename RawOf<VB>::type load_raw(const unsigned char* p, bool yes) {
+    using Raw = typename RawOf<VB>::type;
+    return yes ? *reinterpret_cast<const Raw*>(p) : Raw{};
+}
+
+// U rows of every group of lanes are requested together.
 template <typename T, int VB, int U, int BLOCKS>
-__global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const QkVec v) {
+__global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const __grid_constant__ QkVec v) {
     constexpr int V = VB / sizeof(T);
     using Raw = typename RawOf<VB>::type;
-    __shared__ float weights[kQkMaxDim + 32];      // a lane past the end of a row reads behind it
+    __shared__ __align__(16) float weights[kQkMaxDim + 32];  // a lane past the end of a row reads behind it
     pdl_wait();
     pdl_launch_dependents();
     const bool key = blockIdx.x >= v.side[0].blocks;
     const QkSide& sd = v.side[key];
     const int lane = threadIdx.x & 31, W = 32 / v.G;
-    const Lane n = lane_of<V>(v, lane & (v.G - 1));
+    const Lane n = lane_of<T, VB>(v, lane & (v.G - 1));
     const float inv_d = 1.0f / static_cast<float>(v.d);
     const uint32_t warp = (blockIdx.x - (key ? v.side[0].blocks : 0u)) * 8u + (threadIdx.x >> 5), step = sd.blocks * 8u * W;
     for (int e = threadIdx.x; e < kQkMaxDim + 32; e += 256) weights[e] = sd.w && e < v.d ? sd.w[e] : 1.0f;
     __syncthreads();
     for (uint32_t first = warp * W; first < sd.items; first += step) {
         Item m = item_of<false>(v, sd, first + lane / v.G);
-        // the result is rs * (x_a (w_a c) - x_b (w_b s), x_b (w_b c) + x_a (w_a s))
-        float ac[V], bs[V], bc[V], as[V];
-        load_table<V>(v, n, max(m.pos, 0), bc, as);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {              // neighbours: the lane's two chunks are one run of V pairs
-            const float wa = v.interleaved ? weights[n.a + 2 * i] : weights[n.a + i], wb = v.interleaved ? weights[n.a + 2 * i + 1] : weights[n.b + i];
-            ac[i] = wa * bc[i]; bs[i] = -wb * as[i]; bc[i] = wb * bc[i]; as[i] = wa * as[i];
-        }
-        const bool padding = m.pos < 0;
-        const int count = m.h1 - m.h0;
+        uint64_t c[V], s[V];
+        factors<V>(v, n, max(m.pos, 0), weights, c, s);
+        const int count = m.pos < 0 ? 0 : m.h1 - m.h0;         // padding is neither read nor written
         for (int h = 0; h < sd.per_item; h += U) {
             Raw ra[U], rb[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                ra[u] = Raw{}; rb[u] = Raw{};
-                const T* src = reinterpret_cast<const T*>(m.x + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.x.h);
-                if (h + u < count && n.has_a) ra[u] = *reinterpret_cast<const Raw*>(src + n.a);
-                if (h + u < count && n.has_b) rb[u] = *reinterpret_cast<const Raw*>(src + n.b);
+                ra[u] = load_raw<VB>(m.x + n.at_a, n.has_a && h + u < count);
+                rb[u] = load_raw<VB>(m.x + n.at_b, n.has_b && h + u < count);
+                m.x += sd.x.h;
             }
-            m.x += static_cast<uint64_t>(U) * sd.x.h;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float x[2 * V], y[2 * V];
-                unpack<T, VB>(ra[u], x);
-                unpack<T, VB>(rb[u], x + V);
+                uint64_t x[V], y[V];
+                pairs_of<T, VB>(ra[u], rb[u], x);
                 const float rs = normalizer<V>(v, n, inv_d, x);
-                if (v.interleaved) {
+                const uint64_t r2 = pack2(rs, rs);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float a = x[2 * i] * rs, b = x[2 * i + 1] * rs;
-                        y[2 * i] = fmaf(b, bs[i], a * ac[i]);
-                        y[2 * i + 1] = fmaf(a, as[i], b * bc[i]);
-                    }
-                } else if constexpr (V % 2 == 0) {
-                    const uint64_t r2 = pack2(rs, rs);
-#pragma unroll
-                    for (int i = 0; i < V; i += 2) {
-                        const uint64_t a = fmul2(pack2(x[i], x[i + 1]), r2), b = fmul2(pack2(x[V + i], x[V + i + 1]), r2);
-                        unpack2(ffma2(b, pack2(bs[i], bs[i + 1]), fmul2(a, pack2(ac[i], ac[i + 1]))), y[i], y[i + 1]);
-                        unpack2(ffma2(a, pack2(as[i], as[i + 1]), fmul2(b, pack2(bc[i], bc[i + 1]))), y[V + i], y[V + i + 1]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float a = x[i] * rs, b = x[V + i] * rs;
-                        y[i] = fmaf(b, bs[i], a * ac[i]);
-                        y[V + i] = fmaf(a, as[i], b * bc[i]);
-                    }
-                }
-                if (!v.all_turn) {                 // dims that pass: an infinity must not meet a neighbour, not even times 0
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        if (n.turns && n.pair + i < v.rot / 2) continue;
-                        if (v.interleaved) { y[2 * i] = x[2 * i] * rs * ac[i]; y[2 * i + 1] = x[2 * i + 1] * rs * bc[i]; }
-                        else { y[i] = x[i] * rs * ac[i]; y[V + i] = x[V + i] * rs * bc[i]; }
-                    }
-                }
-                if (h + u < count && !padding) {
-                    T* dst = reinterpret_cast<T*>(m.y + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.y.h);
-                    if (n.has_a) *reinterpret_cast<Raw*>(dst + n.a) = pack<T, VB>(y);
-                    if (n.has_b) *reinterpret_cast<Raw*>(dst + n.b) = pack<T, VB>(y + V);
-                }
+                for (int j = 0; j < V; ++j) x[j] = fmul2(x[j], r2);
+                turn<V>(v, n, x, c, s, y);
+                if (h + u < count) store_pairs<T, VB>(y, m.y, n.at_a, n.at_b, n.has_a, n.has_b);
+                m.y += sd.y.h;
             }
-            m.y += static_cast<uint64_t>(U) * sd.y.h;
         }
     }
 }
 
 template <typename T, int VB, int U, int BLOCKS>
-__global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const QkVec v) {
+__global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __grid_constant__ QkVec v) {
     constexpr int V = VB / sizeof(T);
     using Raw = typename RawOf<VB>::type;
     extern __shared__ float sums[];                // [8][d]
-    __shared__ float weights[kQkMaxDim + 32];
+    __shared__ __align__(16) float weights[kQkMaxDim + 32];
     pdl_wait();
     pdl_launch_dependents();
     const bool key = blockIdx.x >= v.side[0].blocks;
     const QkSide& sd = v.side[key];
     const int lane = threadIdx.x & 31, W = 32 / v.G;
-    const Lane n = lane_of<V>(v, lane & (v.G - 1));
+    const Lane n = lane_of<T, VB>(v, lane & (v.G - 1));
     const float inv_d = 1.0f / static_cast<float>(v.d);
     const uint32_t warp = (blockIdx.x - (key ? v.side[0].blocks : 0u)) * 8u + (threadIdx.x >> 5), step = sd.blocks * 8u * W;
     for (int e = threadIdx.x; e < kQkMaxDim + 32; e += 256) weights[e] = sd.w && e < v.d ? sd.w[e] : 1.0f;
     __syncthreads();
-    float dw[2 * V];
+    uint64_t dw[V];
 #pragma unroll
-    for (int i = 0; i < 2 * V; ++i) dw[i] = 0.0f;
+    for (int j = 0; j < V; ++j) dw[j] = pack2(0.0f, 0.0f);
     for (uint32_t first = warp * W; first < sd.items; first += step) {
         Item m = item_of<true>(v, sd, first + lane / v.G);
         float c[V], s[V];
         load_table<V>(v, n, max(m.pos, 0), c, s);
-        const bool padding = m.pos < 0;
-        const int count = m.h1 - m.h0;
+        const int count = m.h1 - m.h0, live = m.pos < 0 ? 0 : count;
         for (int h = 0; h < sd.per_item; h += U) {
             Raw ra[U], rb[U], ga[U], gb[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                ra[u] = rb[u] = ga[u] = gb[u] = Raw{};
-                if (h + u >= count || padding) continue;       // padding may hold anything: its gradients are 0
-                const T* src = reinterpret_cast<const T*>(m.x + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.x.h);
-                const T* dy = reinterpret_cast<const T*>(m.y + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.y.h);
-                if (n.has_a) { ra[u] = *reinterpret_cast<const Raw*>(src + n.a); ga[u] = *reinterpret_cast<const Raw*>(dy + n.a); }
-                if (n.has_b) { rb[u] = *reinterpret_cast<const Raw*>(src + n.b); gb[u] = *reinterpret_cast<const Raw*>(dy + n.b); }
+            for (int u = 0; u < U; ++u) {          // padding may hold anything: its gradients are 0
+                ra[u] = load_raw<VB>(m.x + n.at_a, n.has_a && h + u < live);
+                rb[u] = load_raw<VB>(m.x + n.at_b, n.has_b && h + u < live);
+                ga[u] = load_raw<VB>(m.y + n.at_a, n.has_a && h + u < live);
+                gb[u] = load_raw<VB>(m.y + n.at_b, n.has_b && h + u < live);
+                m.x += sd.x.h; m.y += sd.y.h;
             }
-            m.x += static_cast<uint64_t>(U) * sd.x.h;
-            m.y += static_cast<uint64_t>(U) * sd.y.h;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                float x[2 * V], y[2 * V];
-                unpack<T, VB>(ra[u], x);
-                unpack<T, VB>(rb[u], x + V);
-                unpack<T, VB>(ga[u], y);
-                unpack<T, VB>(gb[u], y + V);
-                if (n.turns) {
-                    if (v.interleaved) {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            if (!v.all_turn && n.pair + i >= v.rot / 2) continue;
-                            const float a = y[2 * i], b = y[2 * i + 1];
-                            y[2 * i] = fmaf(b, s[i], a * c[i]);
-                            y[2 * i + 1] = fmaf(-a, s[i], b * c[i]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) {
-                            const float a = y[i], b = y[V + i];
-                            y[i] = fmaf(b, s[i], a * c[i]);
-                            y[V + i] = fmaf(-a, s[i], b * c[i]);
-                        }
-                    }
-                }
+                uint64_t x[V], y[V];
+                pairs_of<T, VB>(ra[u], rb[u], x);
+                pairs_of<T, VB>(ga[u], gb[u], y);
+                turn_back<V>(v, n, c, s, y);
                 __syncwarp();
-                const bool live = h + u < count && !padding;
-                const float rs = normalizer<V>(v, n, inv_d, x);
+                float rs = normalizer<V>(v, n, inv_d, x);
+                if (h + u >= live) rs = 0.0f;      // a row of zeros then: with eps = 0 its xhat would be NaN
+                const uint64_t r2 = pack2(rs, rs);
 #pragma unroll
-                for (int i = 0; i < 2 * V; ++i) {
-                    x[i] *= rs;
-                    if (live) dw[i] = fmaf(y[i], x[i], dw[i]); // eps = 0 makes the xhat of a row of zeros NaN
-                    y[i] *= weights[i < V ? n.a + i : n.b + i - V];
+                for (int j = 0; j < V; ++j) {
+                    x[j] = fmul2(x[j], r2);
+                    dw[j] = ffma2(y[j], x[j], dw[j]);
+                    const float w0 = V == 1 || 2 * j < V ? weights[n.a + 2 * j] : weights[n.b + 2 * j - V];
+                    const float w1 = 2 * j + 1 < V ? weights[n.a + 2 * j + 1] : weights[n.b + 2 * j + 1 - V];
+                    y[j] = fmul2(y[j], pack2(w0, w1));
                 }
                 if (v.norm != 0) {
-                    const float sgx = group_sum(lane_dot(y, x), v.G) * inv_d;
-                    const float sg = v.norm == 2 ? group_sum(lane_sum(y), v.G) * inv_d : 0.0f;
+                    const float sgx = -group_sum(lane_dot(y, x), v.G) * inv_d;
+                    const float sg = v.norm == 2 ? -rs * group_sum(lane_sum(y), v.G) * inv_d : 0.0f;
+                    const uint64_t sgx2 = pack2(sgx, sgx), sg2 = pack2(sg, sg);
 #pragma unroll
-                    for (int i = 0; i < 2 * V; ++i) y[i] = rs * (fmaf(-x[i], sgx, y[i]) - sg);
+                    for (int j = 0; j < V; ++j) y[j] = ffma2(ffma2(x[j], sgx2, y[j]), r2, sg2);
                 }
-                if (h + u < count) {
-                    if (padding) {
-#pragma unroll
-                        for (int i = 0; i < 2 * V; ++i) y[i] = 0.0f;
-                    }
-                    T* dst = reinterpret_cast<T*>(m.dx + static_cast<uint64_t>(static_cast<uint32_t>(u)) * sd.dx.h);
-                    if (n.has_a) *reinterpret_cast<Raw*>(dst + n.a) = pack<T, VB>(y);
-                    if (n.has_b) *reinterpret_cast<Raw*>(dst + n.b) = pack<T, VB>(y + V);
-                }
+                if (h + u < count) store_pairs<T, VB>(y, m.dx, n.at_a, n.at_b, n.has_a, n.has_b);
+                m.dx += sd.dx.h;
             }
-            m.dx += static_cast<uint64_t>(U) * sd.dx.h;
         }
     }
     if (!v.partial) return;
     // the rows of a warp, then the warps of the block in order: one line of the workspace per block
-#pragma unroll
-    for (int i = 0; i < 2 * V; ++i)
-        for (int o = v.G; o < 32; o <<= 1) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
     float* mine = sums + (threadIdx.x >> 5) * v.d;
-    if (lane < v.G) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (n.has_a) mine[n.a + i] = dw[i];
-            if (n.has_b) mine[n.b + i] = dw[V + i];
+    for (int j = 0; j < V; ++j) {
+        float t[2];
+        unpack2(dw[j], t[0], t[1]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            for (int o = v.G; o < 32; o <<= 1) t[k] += __shfl_xor_sync(0xffffffffu, t[k], o);
+            const bool in_a = 2 * j + k < V;
+            if (lane < v.G && (in_a ? n.has_a : n.has_b)) mine[in_a ? n.a + 2 * j + k : n.b + 2 * j + k - V] = t[k];
         }
     }
     __syncthreads();
@@ -579,13 +623,16 @@ cudaError_t launch_vec(const QkParams& p, QkVec& v, bool backward, cudaStream_t 
     v.G = 1;
     while (v.G < pairs) v.G *= 2;
     v.all_turn = p.rot == p.d;
+    v.full = v.G * 2 * V == p.d;
     v.table_vec = (reinterpret_cast<uintptr_t>(p.cos_t) | reinterpret_cast<uintptr_t>(p.sin_t)) % 16 == 0 && (p.rot / 2) % 4 == 0 &&
                   (!p.interleaved || (p.rot / 2) % V == 0);
     const int W = 32 / v.G, sms = num_sms();
     const long long tokens = static_cast<long long>(p.B) * p.L;
-    // an item per token where that gives every SM 64 warps or more of them (a few rounds of what is resident), else the heads in
-    // several items, of as many heads as are loaded at once
-    const long long wanted = 64ll * sms * W;
+    // An item is a token with all heads of a side, or, where tokens are few, with some of them.  What an item costs beside its rows
+    // (position, table, factors: about two rows' work) speaks for long ones, even shares of the resident warps for many.
+    // Measured on 16384 tokens x 16 heads of 64 (bf16): forward 34.8 us from 24 items' warps an SM, 36.1 from 96; backward,
+    // whose grid is what is resident, 58.8 and 53.7.
+    const long long wanted = (backward ? 96ll : 24ll) * sms * W;
     long long warps[2];
     for (int k = 0; k < 2; ++k) {
         QkSide& sd = v.side[k];
@@ -609,6 +656,7 @@ cudaError_t launch_vec(const QkParams& p, QkVec& v, bool backward, cudaStream_t 
     }
     v.side[0].blocks = static_cast<uint32_t>(bq); v.side[1].blocks = static_cast<uint32_t>(bk);
     const dim3 grid(static_cast<unsigned>(bq + bk));
+    // rows at once and blocks an SM: as many as the registers hold without spilling
     if (!backward) return launch_pdl(qk_vec_forward_kernel<T, VB, kHeadsAtOnce, V == 8 ? 2 : V == 4 ? 3 : 4>, grid, dim3(256), 0, st, v);
     cudaError_t e = launch_pdl(qk_vec_backward_kernel<T, VB, V == 8 ? 2 : 4, 2>, grid, dim3(256), v.partial ? 8u * p.d * sizeof(float) : 0u, st, v);
     if (e == cudaSuccess && v.partial)
