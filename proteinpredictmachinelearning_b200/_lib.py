@@ -50,7 +50,7 @@ SIGNATURES = {
     "ppml_b200_mul_mat_i8": (_i, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp]),
     "ppml_b200_linear_i8_workspace": (_i64, [_i64, _i]),
     "ppml_b200_linear_i8": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i, _i, _i, _vp, _vp, _i64, _i, _i, _vp, _i64, _vp]),
-    # structures as plain addresses: a caller may pass packed bytes (ops) or byref of the classes above
+    # structures as plain addresses: byref of the classes above
     "ppml_b200_qk_norm_rope": (_i, [_vp] * 11),
     "ppml_b200_qk_norm_rope_backward_workspace": (_i64, [_vp]),
     "ppml_b200_qk_norm_rope_backward": (_i, [_vp] * 15 + [_i64, _vp]),
@@ -98,6 +98,8 @@ SIGNATURES = {
     "ppml_b200_mulmat_stats_dump": (_i, [C.c_char_p, _i]),
 }
 
+TORCH_BINDING_PATH = os.path.join(_HERE, "lib", "ppml_b200_torch.so")
+
 _lib = None
 
 
@@ -117,3 +119,18 @@ def load():
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def load_torch_binding():
+    """The CPython module over the library for torch tensors (csrc/torch_binding.cpp)."""
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries have to be in the process)
+    if not os.path.exists(TORCH_BINDING_PATH):
+        raise ImportError(
+            f"{TORCH_BINDING_PATH} is missing: build it with `python -m proteinpredictmachinelearning_b200.build` "
+            "(there is no CPU or PyTorch fallback for this path)")
+    spec = importlib.util.spec_from_file_location("ppml_b200_torch", TORCH_BINDING_PATH)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module

@@ -1,13 +1,16 @@
-"""Builds libppml_b200.so in-tree with nvcc for sm_100a (no JIT cache, no torch extension)."""
+"""Builds libppml_b200.so in-tree with nvcc for sm_100a (no JIT cache), and ppml_b200_torch.so, the host side of some of its entries
+for torch tensors, with g++ against the installed torch."""
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libppml_b200.so")
+TORCH_BINDING = os.path.join(OUT_DIR, "ppml_b200_torch.so")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -52,6 +55,18 @@ def build(force=False, verbose=False):
         list(ex.map(run, jobs))
     if jobs or not os.path.exists(LIB):
         run([NVCC] + ARCH + ["-shared", "-o", LIB] + objs + ["-Xcompiler", "-fPIC", "-cudart", "static"])
+    binding = os.path.join(CSRC, "torch_binding.cpp")
+    needs = [binding, os.path.join(HERE, "..", "include", "ppml_b200.h")]
+    if force or not os.path.exists(TORCH_BINDING) or any(os.path.getmtime(f) > os.path.getmtime(TORCH_BINDING) for f in needs):
+        import torch
+        root = os.path.dirname(torch.__file__)
+        torch_lib, cuda = os.path.join(root, "lib"), os.path.dirname(os.path.dirname(NVCC))
+        include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include"),
+                   sysconfig.get_paths()["include"]]
+        run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] +
+            [f"-isystem{d}" for d in include] +
+            [binding, "-o", TORCH_BINDING, "-L" + OUT_DIR, "-l:libppml_b200.so", "-L" + torch_lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+             "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
     return LIB
 
 

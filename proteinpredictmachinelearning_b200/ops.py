@@ -3,7 +3,6 @@
 C ABI of libppml_b200.so.  Same names, argument meaning and error behaviour; tensors are torch CUDA
 tensors used only as device memory.  A non-zero status raises RuntimeError."""
 import ctypes as C
-import struct
 
 import numpy as np
 import torch
@@ -184,128 +183,37 @@ def mul_mat_q8_noalloc(W, X, M, wtype=2, c_trans=1, bias=None, out=None):
     return Cout
 
 
-TYPE = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
-
-# The entries from here to qk_norm_rope_backward are called many times for a token, so their host side is kept short: pointers go to
-# the library as plain integers, structures as packed bytes, new tensors come from empty_strided (half the time of empty), messages
-# are only put together for a refusal, and the device is only switched when the tensors' is not the current one.
+_native = None
 
 
-def _raw_stream(index):
-    return torch._C._cuda_getCurrentRawStream(index) or None
-
-
-def _refuse(name, t, want):
-    raise ValueError(f"{name}: {want} wanted, got {tuple(t.shape)} of {t.dtype} on {t.device} with strides {t.stride()}")
-
-
-def _pitch(t, dtype, shape, index, name):
-    """The row pitch of a matrix of that type, shape and device whose rows are contiguous and lie apart."""
-    if t.dtype is dtype and t.shape == shape and t.get_device() == index:
-        s0, s1 = t.stride()
-        M, K = shape
-        if s1 == 1 or K <= 1:
-            if s0 >= K:
-                return s0
-            if M <= 1:
-                return K
-    _refuse(name, t, f"{list(shape)} of {dtype} on cuda:{index}, rows contiguous and apart,")
-
-
-def _vec(t, n, index, name):
-    """The address of n contiguous fp32 values; None for None."""
-    if t is None:
-        return None
-    if t.dtype is torch.float32 and t.shape == (n,) and t.get_device() == index and (t.is_contiguous() or n <= 1):
-        return t.data_ptr()
-    _refuse(name, t, f"{n} contiguous fp32 values on cuda:{index}")
-
-
-def _matrix(x, dtypes, name):
-    """(device index, M, K) of an operand that decides the device of a call."""
-    if x.dim() != 2 or not x.is_cuda or x.dtype not in dtypes:
-        _refuse(name, x, f"a matrix of {[str(t) for t in dtypes]} on the GPU")
-    M, K = x.shape
-    return x.get_device(), M, K
+def _host():
+    """The native host side of the entries below (csrc/torch_binding.cpp): checks of the tensors (ValueError), results and workspaces
+    from torch's allocator, launch on the current stream of the tensors' device."""
+    global _native
+    if _native is None:
+        _native = _lib.load_torch_binding()
+    return _native
 
 
 def quantize_tokens_i8(x, out=None):
     """x [M, K] (fp32, fp16 or bf16; rows contiguous, any pitch) -> (int8 [M, K], fp32 scales [M]): scale = max |x| / 127 of the
     row, q = round(x / scale).  New integers get a row pitch that is a multiple of 16 bytes, which the tensor-core product
-    wants.  Weights [N, K] are quantized the same way, one scale for each output channel."""
-    index, M, K = _matrix(x, TYPE, "x")
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return quantize_tokens_i8(x, out)
-    ld = _pitch(x, x.dtype, (M, K), index, "x")
-    if out is None:
-        dev = x.device
-        ldq = (K + 15) & -16
-        out = q, scale = (torch.empty_strided((M, K), (ldq, 1), dtype=torch.int8, device=dev),
-                          torch.empty_strided((M,), (1,), dtype=torch.float32, device=dev))
-        s = scale.data_ptr()
-    else:
-        q, scale = out
-        ldq, s = _pitch(q, torch.int8, (M, K), index, "q"), _vec(scale, M, index, "scale")
-    rc = _lib.load().ppml_b200_quantize_tokens_i8(x.data_ptr(), TYPE[x.dtype], ld, q.data_ptr(), ldq, s, M, K, _raw_stream(index))
-    if rc:
-        _check(rc, "quantize_tokens_i8")
-    return out
-
-
-def _product_args(like, index, M, K, W, w_scale, bias, gate, act, dtype, path, out):
-    """What both products check and pass alike: the output, the arguments from B to path."""
-    if out is not None:
-        dtype = out.dtype
-    if W.dim() != 2:
-        _refuse("W", W, f"[N, {K}]")
-    if act not in ACT or dtype not in TYPE:
-        raise ValueError(f"act: one of {sorted(ACT)}; type: fp32, fp16 or bf16; got {act!r}, {dtype}")
-    N = W.shape[0]
-    ldb = _pitch(W, torch.int8, (N, K), index, "W")
-    if out is None:
-        out, ldc = torch.empty_strided((M, N), (N, 1), dtype=dtype, device=like.device), N
-    else:
-        ldc = _pitch(out, dtype, (M, N), index, "out")
-    g, ldg = (None, 0) if gate is None else (gate.data_ptr(), _pitch(gate, dtype, (M, N), index, "gate"))
-    return out, (W.data_ptr(), ldb, _vec(w_scale, N, index, "w_scale"), out.data_ptr(), ldc, TYPE[dtype], M, K, N,
-                 None if bias is None else _vec(bias, N, index, "bias"), g, ldg, ACT[act], path)
+    wants.  Weights [N, K] are quantized the same way, one scale for each output channel.  `out`: a pair to write into."""
+    q, scale = out if out is not None else (None, None)
+    return (_native or _host()).quantize_tokens_i8(x, q, scale)
 
 
 def mul_mat_i8(A, a_scale, W, w_scale, bias=None, gate=None, act="none", dtype=torch.float32, path=PATH_AUTO, out=None):
     """act(a_scale[m] * w_scale[n] * sum_k A[m, k] W[n, k] + bias[n]) * gate[m, n]: A int8 [M, K] and W int8 [N, K] with their
-    scales (quantize_tokens_i8), exact int32 sums, fp32 behind them, one rounding to `dtype` (of out and gate)."""
-    index, M, K = _matrix(A, (torch.int8,), "A")
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return mul_mat_i8(A, a_scale, W, w_scale, bias, gate, act, dtype, path, out)
-    lda = _pitch(A, torch.int8, (M, K), index, "A")
-    out, args = _product_args(A, index, M, K, W, w_scale, bias, gate, act, dtype, path, out)
-    rc = _lib.load().ppml_b200_mul_mat_i8(A.data_ptr(), lda, _vec(a_scale, M, index, "a_scale"), *args, _raw_stream(index))
-    if rc:
-        _check(rc, "mul_mat_i8")
-    return out
+    scales (quantize_tokens_i8), exact int32 sums, fp32 behind them, one rounding to `dtype` (of out and gate).  Rows of every
+    matrix are contiguous, at any pitch."""
+    return (_native or _host()).mul_mat_i8(A, a_scale, W, w_scale, bias, gate, act, dtype, path, out)
 
 
 def linear_i8(x, W, w_scale, bias=None, gate=None, act="none", dtype=None, path=PATH_AUTO, out=None):
     """quantize_tokens_i8 and mul_mat_i8 as one call: x [M, K] fp32, fp16 or bf16; the result has x's type unless `dtype` (or
     `out`) says otherwise."""
-    index, M, K = _matrix(x, TYPE, "x")
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return linear_i8(x, W, w_scale, bias, gate, act, dtype, path, out)
-    lib = _lib.load()
-    ld = _pitch(x, x.dtype, (M, K), index, "x")
-    out, args = _product_args(x, index, M, K, W, w_scale, bias, gate, act, dtype or x.dtype, path, out)
-    need = lib.ppml_b200_linear_i8_workspace(M, K)
-    ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=x.device) if need else None
-    rc = lib.ppml_b200_linear_i8(x.data_ptr(), TYPE[x.dtype], ld, *args, None if ws is None else ws.data_ptr(), need, _raw_stream(index))
-    if rc:
-        _check(rc, "linear_i8")
-    return out
-
-
-NORM = {"none": 0, "rms": 1, "layer": 2}
+    return (_native or _host()).linear_i8(x, W, w_scale, bias, gate, act, dtype, path, out)
 
 
 def rope_table(rows, rot, base=10000.0, device="cuda"):
@@ -316,120 +224,23 @@ def rope_table(rows, rot, base=10000.0, device="cuda"):
     return tuple(torch.from_numpy(f(angle).astype(np.float32)).to(device) for f in (np.cos, np.sin))
 
 
-_QK_CFG, _HEADS = struct.Struct("@7if3i4xq"), struct.Struct("@P3q")      # ppml_b200_qk_cfg, ppml_b200_heads
-
-
-def _heads(t, like, name):
-    """The view of `t`, which has the shape, type and device of `like` [B, L, h, d], contiguous d and any other strides; None for no
-    heads."""
-    if t is None or like is None:
-        if t is not like:
-            raise ValueError(f"{name}: missing, or without its input")
-        return None
-    if t is like or t.shape == like.shape and t.dtype is like.dtype and t.get_device() == like.get_device():
-        sb, sl, sh, sd = t.stride()
-        if sd == 1 or t.shape[3] == 1:
-            return _HEADS.pack(t.data_ptr(), sb, sl, sh)
-    _refuse(name, t, f"{list(like.shape)} of {like.dtype} on {like.device} with a contiguous head dim")
-
-
-def _new_heads(x):
-    if x is None:
-        return None
-    B, L, h, d = x.shape
-    return torch.empty_strided((B, L, h, d), (L * h * d, h * d, d, 1), dtype=x.dtype, device=x.device)
-
-
-def _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved):
-    t = Q if Q is not None else K
-    if t is None or t.dim() != 4 or not t.is_cuda or t.dtype not in TYPE:
-        raise ValueError("Q, K: [B, L, heads, d] of fp32, fp16 or bf16 on the GPU are wanted")
-    if norm not in NORM:
-        raise ValueError(f"norm: one of {sorted(NORM)}")
-    B, L, hq, d = t.shape
-    hk, index = 0, t.get_device()
-    if Q is None:
-        hq, hk = 0, hq
-    elif K is not None:
-        shape = K.shape
-        if len(shape) != 4 or K.dtype is not t.dtype or K.get_device() != index or shape[0] != B or shape[1] != L or shape[3] != d:
-            _refuse("K", K, f"[{B}, {L}, heads, {d}] of {t.dtype} on {t.device}")
-        hk = shape[2]
-    rows = rot = pos_b = 0
-    c = s = p = None
-    if cos is not None or sin is not None:
-        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or \
-                sin.dtype is not torch.float32 or cos.get_device() != index or sin.get_device() != index or not cos.is_contiguous() or \
-                not sin.is_contiguous():
-            raise ValueError(f"cos and sin: [rows, rot / 2], contiguous fp32 on {t.device}, are wanted")
-        rows, rot = cos.shape
-        rot *= 2
-        if rot:
-            c, s = cos.data_ptr(), sin.data_ptr()
-    if positions is not None:
-        n = positions.dim()
-        if positions.dtype is not torch.int32 or positions.get_device() != index or n not in (1, 2) or \
-                positions.shape != ((L,) if n == 1 else (B, L)) or (L > 1 and positions.stride(-1) != 1):
-            _refuse("positions", positions, f"[{L}] or [{B}, {L}] int32 on {t.device} with contiguous rows")
-        pos_b, p = positions.stride(0) if n == 2 else 0, positions.data_ptr()
-    cfg = _QK_CFG.pack(B, L, hq, hk, d, TYPE[t.dtype], NORM[norm], eps, rot, 1 if interleaved else 0, rows, pos_b)
-    return index, (cfg, _heads(Q, Q, "Q"), _heads(K, K, "K"), None if q_weight is None else _vec(q_weight, d, index, "q_weight"),
-                   None if k_weight is None else _vec(k_weight, d, index, "k_weight"), c, s, p)
-
-
 def qk_norm_rope(Q, K, q_weight=None, k_weight=None, norm="rms", eps=1e-6, cos=None, sin=None, positions=None, interleaved=False, out=None):
-    """Norm of every head of Q [B, L, hq, d] and K [B, L, hk, d] (any strides with contiguous d: ranges of a fused projection,
-    transposed views of [B, h, L, d]; one of them may be None), times q_weight / k_weight [d], then the rotation of the first
-    2 * cos.shape[1] dims by row `positions` (int32 [B, L] or [L]; None: 0, 1, ...) of cos / sin (rope_table).  A token with a
-    negative position is padding and left alone.  Returns (Q', K'): `out` (tensors of the inputs' shapes and types, any strides; the
-    inputs themselves for a pass in place), or new [B, L, h, d] tensors."""
-    index, args = _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved)
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return qk_norm_rope(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved, out)
-    if out is None:
-        out = _new_heads(Q), _new_heads(K)
-    rc = _lib.load().ppml_b200_qk_norm_rope(*args, _heads(out[0], Q, "out[0]"), _heads(out[1], K, "out[1]"), _raw_stream(index))
-    if rc:
-        _check(rc, "qk_norm_rope")
-    return out
+    """Norm ("rms", "layer" or "none") of every head of Q [B, L, hq, d] and K [B, L, hk, d] (any strides with contiguous d: ranges of
+    a fused projection, transposed views of [B, h, L, d]; one of them may be None), times q_weight / k_weight [d], then the
+    rotation of the first 2 * cos.shape[1] dims by row `positions` (int32 [B, L] or [L]; None: 0, 1, ...) of cos / sin
+    (rope_table).  A token with a negative position is padding and left alone.  Returns (Q', K'): `out` (tensors of the inputs'
+    shapes and types, any strides; the inputs themselves for a pass in place; None for a new one), or new [B, L, h, d] tensors."""
+    q, k = out if out is not None else (None, None)
+    return (_native or _host()).qk_norm_rope(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved, q, k)
 
 
 def qk_norm_rope_backward(Q, K, dQo, dKo, q_weight=None, k_weight=None, norm="rms", eps=1e-6, cos=None, sin=None, positions=None,
                           interleaved=False, out=None):
     """Gradients of qk_norm_rope from its inputs Q, K and the gradients dQo, dKo of its results (their shapes, any strides).  Returns
     a dict: dQ, dK (`out`: tensors to write them into) and, for the weights that are given, dq_weight, dk_weight [d] fp32."""
-    index, args = _qk_args(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved)
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return qk_norm_rope_backward(Q, K, dQo, dKo, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved, out)
-    lib = _lib.load()
-    if out is None:
-        out = _new_heads(Q), _new_heads(K)
-    got = {}
-    if out[0] is not None:
-        got["dQ"] = out[0]
-    if out[1] is not None:
-        got["dK"] = out[1]
-    dqw = dkw = work = None
-    need = 0
-    if q_weight is not None or k_weight is not None:
-        cfg, d = args[0], (Q if Q is not None else K).shape[3]
-        dev = (Q if Q is not None else K).device
-        if q_weight is not None:
-            got["dq_weight"] = w = torch.empty_strided((d,), (1,), dtype=torch.float32, device=dev)
-            dqw = w.data_ptr()
-        if k_weight is not None:
-            got["dk_weight"] = w = torch.empty_strided((d,), (1,), dtype=torch.float32, device=dev)
-            dkw = w.data_ptr()
-        need = lib.ppml_b200_qk_norm_rope_backward_workspace(cfg)
-        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=dev)
-        work = ws.data_ptr()
-    rc = lib.ppml_b200_qk_norm_rope_backward(*args, _heads(dQo, Q, "dQo"), _heads(dKo, K, "dKo"), _heads(out[0], Q, "dQ"),
-                                             _heads(out[1], K, "dK"), dqw, dkw, work, need, _raw_stream(index))
-    if rc:
-        _check(rc, "qk_norm_rope_backward")
-    return got
+    q, k = out if out is not None else (None, None)
+    got = (_native or _host()).qk_norm_rope_backward(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved, dQo, dKo, q, k)
+    return {n: t for n, t in zip(("dQ", "dK", "dq_weight", "dk_weight"), got) if t is not None}
 
 
 def flash_attn_forward_cuda(Q, K, V, bias=None, scale=0.0, causal=False, eps=1e-9, bias_bcast=False, path=PATH_AUTO, out=None,

@@ -291,6 +291,7 @@ def test_in_place_equals_a_new_result(no_device_abort):
         w = rand((d,), 2) + 1
         want = ops.qk_norm_rope(*view(p), q_weight=w, cos=cos, sin=sin)
         mine = p.clone()
+        assert torch.equal(ops.qk_norm_rope(*view(mine), q_weight=w, cos=cos, sin=sin, out=(view(p.clone())[0], None))[1], want[1])
         ops.qk_norm_rope(*view(mine), q_weight=w, cos=cos, sin=sin, out=view(mine))
         assert torch.equal(view(mine)[0], want[0]) and torch.equal(view(mine)[1], want[1]) and torch.equal(mine[..., 8 * d:], p[..., 8 * d:])
         dy = rand((2, 19, 10 * d), 3, dtype)
@@ -517,15 +518,6 @@ def test_bad_arguments_are_refused_on_the_host(lib):
     assert fwd(dict(B=0), Q=None, K=None, Qo=None, Ko=None) == 0 and bwd(dict(L=0), Q=None, K=None, Qo=None, Ko=None, dQ=None, dK=None) == 0
 
 
-def test_packed_structures_are_the_librarys():
-    """ops packs the structures itself: same size and fields as the ctypes classes."""
-    cfg = _lib.QkCfg.from_buffer_copy(ops._QK_CFG.pack(*range(1, 8), 0.5, 9, 10, 11, -(1 << 40)))
-    assert C.sizeof(_lib.QkCfg) == ops._QK_CFG.size
-    assert [getattr(cfg, n) for n, _ in _lib.QkCfg._fields_] == [1, 2, 3, 4, 5, 6, 7, 0.5, 9, 10, 11, -(1 << 40)]
-    v = _lib.Heads.from_buffer_copy(ops._HEADS.pack(1 << 50, 2, -3, 1 << 41))
-    assert C.sizeof(_lib.Heads) == ops._HEADS.size and (v.p, v.sb, v.sl, v.sh) == (1 << 50, 2, -3, 1 << 41)
-
-
 def test_rope_table_in_64_bits():
     cos, sin = ops.rope_table(70000, 64, base=500.0, device="cpu")
     p, i = 69999, np.arange(32)
@@ -549,7 +541,7 @@ def test_wrong_tensors_are_refused():
                 lambda: ops.qk_norm_rope(q, k, q_weight=w[:8]), lambda: ops.qk_norm_rope(q, k, q_weight=w.half()), lambda: ops.qk_norm_rope(q, k, cos=cos),
                 lambda: ops.qk_norm_rope(q, k, cos=cos, sin=sin[:, :4]), lambda: ops.qk_norm_rope(q, k, cos=cos.double(), sin=sin.double()),
                 lambda: ops.qk_norm_rope(q, k, cos=cos, sin=sin, positions=pos.long()), lambda: ops.qk_norm_rope(q, k, cos=cos, sin=sin, positions=pos[:, :4]),
-                lambda: ops.qk_norm_rope(q, k, cos=cos.cpu(), sin=sin.cpu()), lambda: ops.qk_norm_rope(q, k, out=(q, None)),
+                lambda: ops.qk_norm_rope(q, k, cos=cos.cpu(), sin=sin.cpu()), lambda: ops.qk_norm_rope(q, k, eps="1"),
                 lambda: ops.qk_norm_rope(q, None, out=(q, k)), lambda: ops.qk_norm_rope(q, k, out=(q, q)), lambda: ops.qk_norm_rope(q, k, out=(q.half(), k)),
                 lambda: ops.qk_norm_rope_backward(q, k, q, None), lambda: ops.qk_norm_rope_backward(q, k, q, k[:, :3])):
         with pytest.raises(ValueError):
