@@ -37,29 +37,40 @@ __device__ __forceinline__ int i8_quantize(float x, float scale) {
     const float r = rintf(__fdiv_rn(x, scale));
     return static_cast<int>(fminf(fmaxf(r, -127.0f), 127.0f));
 }
-// 1 / scale for i8_quantize4; 0 where its shortcut does not hold
+// 1 / scale for i8_quantize_all; 0 where its shortcut does not hold
 __device__ __forceinline__ float i8_inverse(float scale) { return scale > 1e-30f && scale < 1e30f ? __frcp_rn(scale) : 0.0f; }
-// Four values as packed bytes, the same as i8_quantize.  x * (1 / scale) is within 127 * 2^-23 of the rounded quotient, so the two
-// round alike unless the product lies within 2^-14 of a half: only then is the quotient itself taken.  Adding 1.5 * 2^23 rounds
-// to an integer (half to even) whose low byte is the result.
-__device__ __forceinline__ uint32_t i8_quantize4(const float (&x)[4], float scale, float inv) {
-    constexpr float kRound = 12582912.0f;
-    float t[4], off = 0.0f;
+// N values (a multiple of 4) as packed bytes, the same as i8_quantize.  x * (1 / scale) is within 127 * 2^-23 of the rounded
+// quotient, so the two round alike unless the product lies within 2^-14 of a half: only then is the quotient itself taken.  Adding
+// 1.5 * 2^23 rounds to an integer (half to even) whose low byte is the result.  Two values an instruction.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float r; asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c))); return r;
+}
+template <int N> __device__ __forceinline__ void i8_quantize_all(const float (&x)[N], float scale, float inv, uint32_t (&q)[N / 4]) {
+    const uint64_t inv2 = pack2(inv, inv), round2 = pack2(12582912.0f, 12582912.0f), back2 = pack2(-12582912.0f, -12582912.0f), minus2 = pack2(-1.0f, -1.0f);
+    float off = inv == 0.0f ? 1.0f : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y = x[i] * inv;
-        t[i] = y + kRound;
-        off = fmaxf(off, fabsf(y - (t[i] - kRound)));
-    }
-    if (off > 0.5f - 6.103515625e-5f || inv == 0.0f) {
-        uint32_t v = 0;
+    for (int i = 0; i < N; i += 4) {
+        uint32_t b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v |= (static_cast<uint32_t>(i8_quantize(x[i], scale)) & 255u) << (8 * i);
-        return v;
+        for (int k = 0; k < 4; k += 2) {
+            const uint64_t y = fmul2(pack2(x[i + k], x[i + k + 1]), inv2), t = fadd2(y, round2);
+            float d0, d1, t0, t1;
+            unpack2(ffma2(fadd2(t, back2), minus2, y), d0, d1);
+            unpack2(t, t0, t1);
+            off = max3_abs(off, d0, d1);
+            b[k] = __float_as_uint(t0); b[k + 1] = __float_as_uint(t1);
+        }
+        q[i / 4] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
-    const uint32_t lo = __byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040);
-    const uint32_t hi = __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040);
-    return __byte_perm(lo, hi, 0x5410);
+    if (off > 0.5f - 6.103515625e-5f) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            uint32_t v = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v |= (static_cast<uint32_t>(i8_quantize(x[i + k], scale)) & 255u) << (8 * k);
+            q[i / 4] = v;
+        }
+    }
 }
 
 // 16 bytes of a row of x
@@ -91,11 +102,7 @@ template <typename T> __device__ __forceinline__ void unpack_vec(const uint4& v,
 template <typename T> __device__ __forceinline__ void quantize_vec(const uint4& v, float scale, float inv, uint32_t (&q)[Vec16<T>::kN / 4]) {
     float x[Vec16<T>::kN];
     unpack_vec<T>(v, x);
-#pragma unroll
-    for (int i = 0; i < Vec16<T>::kN / 4; ++i) {
-        const float f[4] = {x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
-        q[i] = i8_quantize4(f, scale, inv);
-    }
+    i8_quantize_all(x, scale, inv, q);
 }
 
 // The activations of act_scalar with sigmoid, SiLU and GELU through the hardware's exp2 and reciprocal (about 2 ulp each, the

@@ -149,6 +149,13 @@ __device__ __forceinline__ void store_any(const I8Product& p, const uint32_t (&s
         }
     }
 }
+// The gates of a chunk are requested before its sums are there (no register waits for them).
+template <typename T>
+__device__ __forceinline__ void prefetch_gates(const I8Product& p, long long t0, int left, long long n, bool n_ok) {
+    if (!p.gate || !n_ok) return;
+    const T* g = static_cast<const T*>(p.gate) + t0 * p.ld_gate + n;
+    for (int j = 0; j < min(left, 32); ++j, g += p.ld_gate) asm volatile("prefetch.global.L1 [%0];" ::"l"(g));
+}
 template <typename T>
 __device__ __forceinline__ void store_chunk(const I8Product& p, const uint32_t (&sum)[32], float* scale_buf, float scale, long long t0, int left,
                                             long long n, bool n_ok, float b_scale, float bias, int lane) {
@@ -284,6 +291,7 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             for (int k = 0; k < 2; ++k) {
                 const int c = (part + k * kEpiParts) * 32 + lane;
                 scale[k] = c < cols ? q.p.a_scale[t0 + c] : 0.0f;
+                prefetch_gates<T>(q.p, t0 + c - lane, cols - (c - lane), n, n_ok);
             }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull(acc), aph, cta_abort, q.err, 0x840 | acc))) break;
             tc_fence_after();
@@ -394,6 +402,7 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     float* scale_buf = scales + (warp - kFirstEpi) * 32;
     const float scale = warp >= kFirstEpi && part * 32 + lane < cols ? q.p.a_scale[t0 + part * 32 + lane] : 0.0f;
     if (warp >= kFirstEpi) {
+        prefetch_gates<T>(q.p, t0 + part * 32, cols - part * 32, n, n_ok);
         if (__all_sync(0xffffffffu, mbar_wait(tfull, 0, cta_abort, q.err, 0x940))) {
             tc_fence_after();
             const int c = part * 32;               // bn <= 128: at most one chunk per warp
