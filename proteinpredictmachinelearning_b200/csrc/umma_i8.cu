@@ -106,66 +106,107 @@ __device__ __forceinline__ void issue_block(bool lead, uint32_t d, uint64_t desc
 }
 
 // ---- epilogue of 32 tokens x this lane's channel ----
-// All 32 tokens, no activation, no gate: straight code, the row pitch in 32 bits (one multiply-add per address).
-template <typename T>
-__device__ __forceinline__ void store_plain(const uint32_t (&sum)[32], const float* scale_buf, T* c, uint32_t ldc, float b_scale, float bias) {
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __nv_bfloat16) { const __nv_bfloat162 t = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
+__device__ __forceinline__ uint32_t narrow2(float a, float b, __half) { const __half2 t = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
+
+// Gates of 32 tokens, requested before their sums are there.
+template <typename T, int MORE> struct Gates {
+    uint32_t w[MORE < 2 ? 1 : sizeof(T) == 2 ? 16 : 32];
+    __device__ __forceinline__ void load(const I8Product& p, long long t0, int left, long long n) {
+        if (MORE < 2 || n >= p.N) return;
+        const T* g = static_cast<const T*>(p.gate) + t0 * p.ld_gate + n;
 #pragma unroll
-    for (int j0 = 0; j0 < 32; j0 += 4) {
-        const float4 s = reinterpret_cast<const float4*>(scale_buf)[j0 / 4];
-        const float f[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            c[static_cast<uint64_t>(ldc) * static_cast<uint32_t>(j0 + j)] =
-                from_f32<T>(fmaf(static_cast<float>(static_cast<int>(sum[j0 + j])) * f[j], b_scale, bias));
-    }
-}
-// Everything else.
-template <typename T>
-__device__ __forceinline__ void store_any(const I8Product& p, const uint32_t (&sum)[32], const float* scale_buf, int left, T* c, const T* g,
-                                       float b_scale, float bias) {
-#pragma unroll
-    for (int j0 = 0; j0 < 32; j0 += 8) {
-        if (j0 >= left) return;
-        float y[8], s[8];
-        *reinterpret_cast<float4*>(s) = reinterpret_cast<const float4*>(scale_buf)[j0 / 4];
-        *reinterpret_cast<float4*>(s + 4) = reinterpret_cast<const float4*>(scale_buf)[j0 / 4 + 1];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = fmaf(static_cast<float>(static_cast<int>(sum[j0 + j])) * s[j], b_scale, bias);
-        if (p.act != 0) {
-#pragma unroll
-            for (int j = 0; j < 8; j += 4) *reinterpret_cast<float4*>(y + j) = i8_act4(p.act, make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]));
-        }
-        if (g) {
-            float gv[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) { gv[j] = j0 + j < left ? to_f32(*g) : 0.0f; g += p.ld_gate; }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] *= gv[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (j0 + j < left) *c = from_f32<T>(y[j]);
-            c += p.ldc;
+        for (int j = 0; j < 32; ++j, g += p.ld_gate) {
+            if constexpr (sizeof(T) == 4) {
+                w[j] = j < left ? *reinterpret_cast<const uint32_t*>(g) : 0u;
+            } else {
+                const uint32_t v = j < left ? *reinterpret_cast<const uint16_t*>(g) : 0u;
+                w[j / 2] = j & 1 ? w[j / 2] | v << 16 : v;
+            }
         }
     }
-}
-// The gates of a chunk are requested before its sums are there (no register waits for them).
-template <typename T>
-__device__ __forceinline__ void prefetch_gates(const I8Product& p, long long t0, int left, long long n, bool n_ok) {
-    if (!p.gate || !n_ok) return;
-    const T* g = static_cast<const T*>(p.gate) + t0 * p.ld_gate + n;
-    for (int j = 0; j < min(left, 32); ++j, g += p.ld_gate) asm volatile("prefetch.global.L1 [%0];" ::"l"(g));
-}
-template <typename T>
-__device__ __forceinline__ void store_chunk(const I8Product& p, const uint32_t (&sum)[32], float* scale_buf, float scale, long long t0, int left,
-                                            long long n, bool n_ok, float b_scale, float bias, int lane) {
+    __device__ __forceinline__ float at(int j) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[j]);
+        else { const uint16_t v = static_cast<uint16_t>(j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu); return to_f32(*reinterpret_cast<const T*>(&v)); }
+    }
+};
+
+// The sums of `left` tokens (>= 32: all) from t0 on in this lane's channel n become results and go to C, eight tokens at a time.
+// MORE: 0 nothing follows, 1 an activation, 2 a gate (and perhaps an activation): instances of their own, because the registers of the
+// gates and the code of the five activations cost the plain ones a fifth of their time.  16-bit results in rows on 4 bytes go
+// out two channels a lane: neighbouring lanes exchange one of two tokens, an even lane keeps its first token and takes the
+// neighbour's, an odd one the second.
+template <typename T, int MORE>
+__device__ __forceinline__ void finish_chunk(const I8Product& p, const uint32_t (&sum)[32], const Gates<T, MORE>& gate, float* scale_buf, float scale,
+                                             long long t0, int left, long long n, float b_scale, float bias, int lane) {
     __syncwarp();
     scale_buf[lane] = scale;
     __syncwarp();
-    if (n_ok) {
-        T* c = static_cast<T*>(p.C) + t0 * p.ldc + n;
-        if (left >= 32 && p.act == 0 && !p.gate && p.ldc <= 0x7fffffffLL) store_plain<T>(sum, scale_buf, c, static_cast<uint32_t>(p.ldc), b_scale, bias);
-        else store_any<T>(p, sum, scale_buf, left, c, p.gate ? static_cast<const T*>(p.gate) + t0 * p.ld_gate + n : nullptr, b_scale, bias);
+    const uint64_t b2 = pack2(b_scale, b_scale), bias2 = pack2(bias, bias);
+    T* c = static_cast<T*>(p.C) + t0 * p.ldc + n;
+    const uint64_t ldc = static_cast<uint32_t>(p.ldc);         // below 2^32 (the launcher's condition): one multiply-add per address
+    auto results = [&](int j0, float (&y)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            const float4 s = reinterpret_cast<const float4*>(scale_buf)[(j0 + j) / 4];
+            auto f = [&](int i) { return static_cast<float>(static_cast<int>(sum[j0 + j + i])); };
+            unpack2(ffma2(fmul2(pack2(f(0), f(1)), pack2(s.x, s.y)), b2, bias2), y[j], y[j + 1]);
+            unpack2(ffma2(fmul2(pack2(f(2), f(3)), pack2(s.z, s.w)), b2, bias2), y[j + 2], y[j + 3]);
+        }
+        if constexpr (MORE > 0) i8_act_all(p.act, y);
+        if constexpr (MORE == 2) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] *= gate.at(j0 + j);
+        }
+    };
+    const bool odd = lane & 1;
+    uint32_t* to = reinterpret_cast<uint32_t*>(c + (odd ? ldc - 1 : 0));       // two channels of one token
+    const uint32_t pick = odd ? 0x3276 : 0x5410;
+    auto store_paired = [&](int j0, const float (&y)[8]) {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const uint32_t own = narrow2(y[j], y[j + 1], T()), other = __shfl_xor_sync(0xffffffffu, own, 1);
+                to[ldc / 2 * (j0 + j)] = __byte_perm(own, other, pick);
+            }
+        }
+    };
+    const bool paired = sizeof(T) == 2 && left >= 32 && n - lane + 32 <= p.N && ((reinterpret_cast<uintptr_t>(p.C) >> 1 | p.ldc) & 1) == 0;
+    if (MORE > 0) {                                // one copy of the activations
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            float y[8];
+            results(j0, y);
+            if (paired) {
+                store_paired(j0, y);
+            } else if (n < p.N) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j0 + j < left) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
+            }
+        }
+    } else if (paired) {
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y); store_paired(j0, y); }
+    } else if (n < p.N) {
+        if (left >= 32) {
+#pragma unroll
+            for (int j0 = 0; j0 < 32; j0 += 8) {
+                float y[8];
+                results(j0, y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
+            }
+        } else {
+#pragma unroll
+            for (int j0 = 0; j0 < 32; j0 += 8) {
+                float y[8];
+                results(j0, y);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j0 + j < left) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
+            }
+        }
     }
     __syncwarp();
 }
@@ -179,7 +220,7 @@ __device__ __noinline__ void wait_for_copies() {
 // Persistent: a CTA (CG = 1) or a pair of CTAs (CG = 2: 256 channels, each CTA holding half of the weight rows and half of the
 // token rows of a stage) takes every gridDim-th tile; two accumulators in TMEM, so that a tile's epilogue runs under the
 // next tile's MMAs.
-template <typename T, int CG>
+template <typename T, int CG, int MORE>
 __global__ void __launch_bounds__(kThreadsI8, 1)
 i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const I8Tc q) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];      // no static shared memory: it starts on the swizzle's 1024 bytes
@@ -287,12 +328,13 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             const long long rest = q.p.M - t0;
             const int cols = static_cast<int>(rest < q.bn ? rest : q.bn);
             float scale[2];                        // of the chunks this warp will read, requested before the wait
+            Gates<T, MORE> gate;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int c = (part + k * kEpiParts) * 32 + lane;
                 scale[k] = c < cols ? q.p.a_scale[t0 + c] : 0.0f;
-                prefetch_gates<T>(q.p, t0 + c - lane, cols - (c - lane), n, n_ok);
             }
+            gate.load(q.p, t0 + part * 32, cols - part * 32, n);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull(acc), aph, cta_abort, q.err, 0x840 | acc))) break;
             tc_fence_after();
             const uint32_t d = tmem + acc * (q.tmem_cols / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -301,6 +343,7 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 const int c = (part + k * kEpiParts) * 32;
                 uint32_t r[32];
                 if (c < cols) {
+                    if (k == 1) gate.load(q.p, t0 + c, cols - c, n);
                     __syncwarp();
                     tmem_ld32(d + c, r);
                     tmem_ld_wait();
@@ -311,7 +354,7 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                     __syncwarp();
                     if (lane == 0) { if (CG == 2) mbar_arrive_cluster(map_to(tempty(acc), 0)); else mbar_arrive(tempty(acc)); }
                 }
-                if (c < cols) store_chunk<T>(q.p, r, scale_buf, scale[k], t0 + c, cols - c, n, n_ok, bs, bias, lane);
+                if (c < cols) finish_chunk<T, MORE>(q.p, r, gate, scale_buf, scale[k], t0 + c, cols - c, n, bs, bias, lane);
             }
             if (++acc == 2) { acc = 0; aph ^= 1u; }
         }
@@ -328,7 +371,7 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
 
 // Few tiles: one tile per cluster of `parts` CTAs, each of which sums its share of K; the int32 partial sums meet in shared
 // memory, every CTA finishing its share of the tokens.
-template <typename T>
+template <typename T, int MORE>
 __global__ void __launch_bounds__(kThreadsI8, 1)
 i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const I8Tc q, const int parts) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];      // no static shared memory: it starts on the swizzle's 1024 bytes
@@ -401,8 +444,9 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     const float bs = n_ok ? q.p.b_scale[n] : 0.0f, bias = n_ok && q.p.bias ? q.p.bias[n] : 0.0f;
     float* scale_buf = scales + (warp - kFirstEpi) * 32;
     const float scale = warp >= kFirstEpi && part * 32 + lane < cols ? q.p.a_scale[t0 + part * 32 + lane] : 0.0f;
+    Gates<T, MORE> gate;
     if (warp >= kFirstEpi) {
-        prefetch_gates<T>(q.p, t0 + part * 32, cols - part * 32, n, n_ok);
+        if (parts == 1) gate.load(q.p, t0 + part * 32, cols - part * 32, n);
         if (__all_sync(0xffffffffu, mbar_wait(tfull, 0, cta_abort, q.err, 0x940))) {
             tc_fence_after();
             const int c = part * 32;               // bn <= 128: at most one chunk per warp
@@ -412,7 +456,7 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
                 tmem_ld_wait();
                 if (parts == 1) {
-                    store_chunk<T>(q.p, r, scale_buf, scale, t0 + c, cols - c, n, n_ok, bs, bias, lane);
+                    finish_chunk<T, MORE>(q.p, r, gate, scale_buf, scale, t0 + c, cols - c, n, bs, bias, lane);
                 } else {                           // the stages are free: every load has landed and every MMA has read
                     uint32_t* buf = reinterpret_cast<uint32_t*>(gen) + c * kRowsA + quarter * 32 + lane;
 #pragma unroll
@@ -430,14 +474,16 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 uint32_t v[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = 0;
-                const float s = lane < min(8, cols - c) ? q.p.a_scale[t0 + c + lane] : 0.0f;
+                const int left = min(8, cols - c);
+                const float s = lane < left ? q.p.a_scale[t0 + c + lane] : 0.0f;
+                gate.load(q.p, t0 + c, left, n);
                 const uint32_t at = base + static_cast<uint32_t>((c * kRowsA + quarter * 32 + lane) * 4);
                 for (int r = 0; r < parts; ++r) {
                     const uint32_t there = map_to(at, static_cast<uint32_t>((rank + r) % parts));
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[j] += ld_cluster_s32(there + j * kRowsA * 4);
                 }
-                store_chunk<T>(q.p, v, scale_buf, s, t0 + c, min(8, cols - c), n, n_ok, bs, bias, lane);
+                finish_chunk<T, MORE>(q.p, v, gate, scale_buf, s, t0 + c, left, n, bs, bias, lane);
             }
         }
     }
@@ -499,7 +545,7 @@ Plan choose(const I8Product& p) {
     return plan;
 }
 
-template <typename T>
+template <typename T, int MORE>
 int launch_t(const I8Product& p, const Plan& plan, cudaStream_t st) {
     const int cg = plan.pair == 2 ? 2 : 1;
     I8Tc q{};
@@ -521,24 +567,33 @@ int launch_t(const I8Product& p, const Plan& plan, cudaStream_t st) {
     cudaError_t e;
     if (plan.pair == 0) {
         q.tmem_cols = pow2_at_least(plan.bn, 32);
-        e = launch_cluster<i8_parts_kernel<T>>(q.tiles_n * q.tiles_t * plan.parts, plan.parts, smem, st, tmW, tmA, q, plan.parts);
+        e = launch_cluster<i8_parts_kernel<T, MORE>>(q.tiles_n * q.tiles_t * plan.parts, plan.parts, smem, st, tmW, tmA, q, plan.parts);
     } else {
         q.tmem_cols = 2 * pow2_at_least(plan.bn, 32);
         const int units = q.tiles_n * q.tiles_t, most = num_sms() / cg, groups = units < most ? units : most;
-        e = cg == 2 ? launch_cluster<i8_tiles_kernel<T, 2>>(groups * 2, 2, smem, st, tmW, tmA, q)
-                    : launch_cluster<i8_tiles_kernel<T, 1>>(groups, 1, smem, st, tmW, tmA, q);
+        e = cg == 2 ? launch_cluster<i8_tiles_kernel<T, 2, MORE>>(groups * 2, 2, smem, st, tmW, tmA, q)
+                    : launch_cluster<i8_tiles_kernel<T, 1, MORE>>(groups, 1, smem, st, tmW, tmA, q);
     }
     if (e != cudaSuccess) { cudaGetLastError(); return ST_LAUNCH; }
     return ST_OK;
 }
 
+template <typename T>
+int launch_more(const I8Product& p, const Plan& plan, cudaStream_t st) {
+    return p.gate ? launch_t<T, 2>(p, plan, st) : p.act ? launch_t<T, 1>(p, plan, st) : launch_t<T, 0>(p, plan, st);
+}
+
 }  // namespace
 
 int launch_umma_i8(const I8Product& p, cudaStream_t st) {
+    if (p.ldc > UINT32_MAX) return ST_UNSUPPORTED_PATH;
     if ((reinterpret_cast<uintptr_t>(p.A) | reinterpret_cast<uintptr_t>(p.B) | p.lda | p.ldb) & 15) return ST_UNSUPPORTED_PATH;
     const Plan plan = choose(p);
-    return p.c_type == kTypeF32 ? launch_t<float>(p, plan, st)
-                                : p.c_type == kTypeF16 ? launch_t<__half>(p, plan, st) : launch_t<__nv_bfloat16>(p, plan, st);
+    switch (p.c_type) {
+        case kTypeF32: return launch_more<float>(p, plan, st);
+        case kTypeF16: return launch_more<__half>(p, plan, st);
+        default: return launch_more<__nv_bfloat16>(p, plan, st);
+    }
 }
 
 }  // namespace ppml_b200
