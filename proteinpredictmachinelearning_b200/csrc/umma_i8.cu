@@ -369,8 +369,8 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     if (warp == 1) tmem_free_cg<CG>(tmem, q.tmem_cols);
 }
 
-// Few tiles: one tile per cluster of `parts` CTAs, each of which sums its share of K; the int32 partial sums meet in shared
-// memory, every CTA finishing its share of the tokens.
+// Few tiles and a long K: one tile per cluster of `parts` CTAs (2, 4, 8), each of which sums its share of K; the int32 partial sums
+// meet in shared memory, every CTA finishing its share of the tokens.
 template <typename T, int MORE>
 __global__ void __launch_bounds__(kThreadsI8, 1)
 i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const I8Tc q, const int parts) {
@@ -387,7 +387,7 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     float* scales = reinterpret_cast<float*>(tail + kBarBytes);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = parts > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int rank = static_cast<int>(cluster_rank());
     const int tile = blockIdx.x / parts, tn = tile / q.tiles_t, tt = tile - tn * q.tiles_t;
     const int kb0 = static_cast<int>(static_cast<long long>(q.kblocks) * rank / parts);
     const int kb1 = static_cast<int>(static_cast<long long>(q.kblocks) * (rank + 1) / parts);
@@ -443,10 +443,7 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     const bool n_ok = n < q.p.N;
     const float bs = n_ok ? q.p.b_scale[n] : 0.0f, bias = n_ok && q.p.bias ? q.p.bias[n] : 0.0f;
     float* scale_buf = scales + (warp - kFirstEpi) * 32;
-    const float scale = warp >= kFirstEpi && part * 32 + lane < cols ? q.p.a_scale[t0 + part * 32 + lane] : 0.0f;
-    Gates<T, MORE> gate;
     if (warp >= kFirstEpi) {
-        if (parts == 1) gate.load(q.p, t0 + part * 32, cols - part * 32, n);
         if (__all_sync(0xffffffffu, mbar_wait(tfull, 0, cta_abort, q.err, 0x940))) {
             tc_fence_after();
             const int c = part * 32;               // bn <= 128: at most one chunk per warp
@@ -455,36 +452,32 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 __syncwarp();
                 tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
                 tmem_ld_wait();
-                if (parts == 1) {
-                    finish_chunk<T, MORE>(q.p, r, gate, scale_buf, scale, t0 + c, cols - c, n, bs, bias, lane);
-                } else {                           // the stages are free: every load has landed and every MMA has read
-                    uint32_t* buf = reinterpret_cast<uint32_t*>(gen) + c * kRowsA + quarter * 32 + lane;
+                // the stages are free: every load has landed and every MMA has read
+                uint32_t* buf = reinterpret_cast<uint32_t*>(gen) + c * kRowsA + quarter * 32 + lane;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) buf[j * kRowsA] = r[j];
-                }
+                for (int j = 0; j < 32; ++j) buf[j * kRowsA] = r[j];
             }
         }
     }
-    if (parts > 1) {
-        __syncwarp();
-        cluster_sync_all();
-        if (warp >= kFirstEpi) {
-            // tokens in chunks of 8, dealt to the CTAs and within a CTA to its four groups of warps
-            for (int c = (rank + part * parts) * 8; c < cols; c += 8 * parts * kEpiParts) {
-                uint32_t v[32];
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= kFirstEpi) {
+        // tokens in chunks of 8, dealt to the CTAs and within a CTA to its four groups of warps
+        for (int c = (rank + part * parts) * 8; c < cols; c += 8 * parts * kEpiParts) {
+            uint32_t v[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0;
-                const int left = min(8, cols - c);
-                const float s = lane < left ? q.p.a_scale[t0 + c + lane] : 0.0f;
-                gate.load(q.p, t0 + c, left, n);
-                const uint32_t at = base + static_cast<uint32_t>((c * kRowsA + quarter * 32 + lane) * 4);
-                for (int r = 0; r < parts; ++r) {
-                    const uint32_t there = map_to(at, static_cast<uint32_t>((rank + r) % parts));
+            for (int j = 0; j < 32; ++j) v[j] = 0;
+            const int left = min(8, cols - c);
+            const float s = lane < left ? q.p.a_scale[t0 + c + lane] : 0.0f;
+            Gates<T, MORE> gate;
+            gate.load(q.p, t0 + c, left, n);
+            const uint32_t at = base + static_cast<uint32_t>((c * kRowsA + quarter * 32 + lane) * 4);
+            for (int r = 0; r < parts; ++r) {
+                const uint32_t there = map_to(at, static_cast<uint32_t>((rank + r) % parts));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] += ld_cluster_s32(there + j * kRowsA * 4);
-                }
-                finish_chunk<T, MORE>(q.p, v, gate, scale_buf, s, t0 + c, left, n, bs, bias, lane);
+                for (int j = 0; j < 8; ++j) v[j] += ld_cluster_s32(there + j * kRowsA * 4);
             }
+            finish_chunk<T, MORE>(q.p, v, gate, scale_buf, s, t0 + c, left, n, bs, bias, lane);
         }
     }
     __syncwarp();
@@ -492,7 +485,7 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     __syncthreads();
     if (*cta_abort && threadIdx.x == 0) wait_for_copies();
     __syncwarp();
-    if (parts > 1) cluster_sync_all();
+    cluster_sync_all();
     tc_fence_after();
     if (warp == 1) { tmem_relinquish(); tmem_dealloc(tmem, q.tmem_cols); }
 }
@@ -523,26 +516,40 @@ cudaError_t launch_cluster(int grid, int cluster, size_t smem, cudaStream_t st, 
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-struct Plan { int pair, bn, parts; };              // pair: 0 parts kernel, 1 persistent single CTAs, 2 persistent pairs
+// How a product is cut: `pair` 1 persistent single CTAs, 2 persistent pairs, 0 one tile per cluster of `parts` CTAs.
+struct Plan { int pair, bn, parts; };
 
+// The cut with the shortest estimate, in cycles, for the busiest CTA.  A stage of 128 k takes 2.1 cycles a row (the rate at which
+// tiles come out of L2: a pair fetches half of the token rows each), a tile's epilogue 8 a token, a tile 400 besides, a pair's
+// hand-shakes 800; parts of K cost 1600 + 49 a token for the partial sums' way through shared memory.  Fitted to the following, best
+// against other cuts (us, bf16 results): 408 x 1024 -> 1024 32 tokens a tile 4.5, 128 in four parts 6.8; 200 x 8192 -> 1024 64 in four
+// parts 9.2, 32 in two 11.6; 1999 x 1000 -> 777 96 6.4, 128 6.9; 8192 x 256 -> 512 single 5.4, pairs 6.2; 5000 x 4000 -> 1000
+// pairs 24.4, single 30.6; 65536 x 256 -> 256 tiles of 256 13.5, of 128 14.5.
 Plan choose(const I8Product& p) {
-    const long long sms = num_sms();
-    const int kblocks = (p.K + 127) / 128;
-    const long long tn = (p.N + 127) / 128;
-    auto tt = [&](int bn) { return (p.M + static_cast<long long>(bn) - 1) / bn; };
-    Plan plan{0, 0, 1};
-    const int cap = p.M >= 128 ? 128 : (p.M + 15) / 16 * 16;
-    if (tn * tt(128) > sms) {
-        plan.pair = p.N > 128 ? 2 : 1;
-        plan.bn = 256;
-        while (plan.bn > 64 && (tn + plan.pair - 1) / plan.pair * tt(plan.bn) * plan.pair < 4 * sms && kblocks <= 8) plan.bn /= 2;
-        return plan;
+    const long long sms = num_sms(), kb = (p.K + 127) / 128, M = p.M;
+    Plan best{1, 256, 1};
+    long long least = INT64_MAX;
+    auto consider = [&](Plan plan) {
+        const int cg = plan.pair == 2 ? 2 : 1;
+        const long long tn = (p.N + 128ll * cg - 1) / (128 * cg), tt = (M + plan.bn - 1) / plan.bn, units = tn * tt * plan.parts;
+        const long long rounds = (units + sms / cg - 1) / (sms / cg), steps = (kb + plan.parts - 1) / plan.parts;
+        const long long fill = steps * (128 + plan.bn / cg) * 21 / 10;
+        const long long cost = rounds * (fill + (plan.pair == 0 ? 1600 + 49 * plan.bn : 8 * plan.bn + 400 + (cg == 2 ? 800 : 0)));
+        if (cost < least) { least = cost; best = plan; }
+    };
+    const int most = M >= 256 ? 256 : static_cast<int>((M + 15) / 16 * 16);        // whole tiles of tokens for small M
+    for (int bn = most < 32 ? most : 32; bn <= most; bn += bn < 32 ? 16 : 32) {
+        consider({1, bn, 1});
+        if (p.N > 128 && bn >= 64) consider({2, bn, 1});
+        if (bn <= 128)
+            for (int parts = 2; parts <= 8 && 2 * parts <= kb; parts *= 2) consider({0, bn, parts});
     }
-    plan.bn = cap;
-    while (plan.bn > 32 && tn * tt(plan.bn) * 2 <= sms && kblocks < 8) plan.bn = (plan.bn / 2 + 15) / 16 * 16;
-    const long long tiles = tn * tt(plan.bn);
-    while (plan.parts < 8 && tiles * plan.parts * 2 <= sms && kblocks >= 4 * plan.parts) plan.parts *= 2;
-    return plan;
+    if (most > 32 && most % 32 != 0) {             // one tile of exactly M tokens
+        consider({1, most, 1});
+        if (most <= 128)
+            for (int parts = 2; parts <= 8 && 2 * parts <= kb; parts *= 2) consider({0, most, parts});
+    }
+    return best;
 }
 
 template <typename T, int MORE>
