@@ -467,17 +467,20 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const __gri
     __syncthreads();
     for (uint32_t first = warp * W; first < sd.items; first += step) {
         Item m = item_of<false>(v, sd, first + lane / v.G);
-        uint64_t c[V], s[V];
-        factors<V>(v, n, max(m.pos, 0), weights, c, s);
         const int count = m.pos < 0 ? 0 : m.h1 - m.h0;         // padding is neither read nor written
-        for (int h = 0; h < sd.per_item; h += U) {
-            Raw ra[U], rb[U];
+        Raw ra[U], rb[U];
+        auto load = [&](int h) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 ra[u] = load_raw<VB>(m.x + n.at_a, n.has_a && h + u < count);
                 rb[u] = load_raw<VB>(m.x + n.at_b, n.has_b && h + u < count);
                 m.x += sd.x.h;
             }
+        };
+        load(0);                                               // before the table, whose row waits for the position
+        uint64_t c[V], s[V];
+        factors<V>(v, n, max(m.pos, 0), weights, c, s);
+        for (int h = 0;;) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 uint64_t x[V], y[V];
@@ -490,6 +493,9 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const __gri
                 if (h + u < count) store_pairs<T, VB>(y, m.y, n.at_a, n.at_b, n.has_a, n.has_b);
                 m.y += sd.y.h;
             }
+            h += U;
+            if (h >= sd.per_item) break;
+            load(h);
         }
     }
 }
@@ -515,11 +521,9 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
     for (int j = 0; j < V; ++j) dw[j] = pack2(0.0f, 0.0f);
     for (uint32_t first = warp * W; first < sd.items; first += step) {
         Item m = item_of<true>(v, sd, first + lane / v.G);
-        float c[V], s[V];
-        load_table<V>(v, n, max(m.pos, 0), c, s);
         const int count = m.h1 - m.h0, live = m.pos < 0 ? 0 : count;
-        for (int h = 0; h < sd.per_item; h += U) {
-            Raw ra[U], rb[U], ga[U], gb[U];
+        Raw ra[U], rb[U], ga[U], gb[U];
+        auto load = [&](int h) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {          // padding may hold anything: its gradients are 0
                 ra[u] = load_raw<VB>(m.x + n.at_a, n.has_a && h + u < live);
@@ -528,6 +532,11 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
                 gb[u] = load_raw<VB>(m.y + n.at_b, n.has_b && h + u < live);
                 m.x += sd.x.h; m.y += sd.y.h;
             }
+        };
+        load(0);                                   // before the table, whose row waits for the position
+        float c[V], s[V];
+        load_table<V>(v, n, max(m.pos, 0), c, s);
+        for (int h = 0;;) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 uint64_t x[V], y[V];
@@ -556,6 +565,9 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
                 if (h + u < count) store_pairs<T, VB>(y, m.dx, n.at_a, n.at_b, n.has_a, n.has_b);
                 m.dx += sd.dx.h;
             }
+            h += U;
+            if (h >= sd.per_item) break;
+            load(h);
         }
     }
     if (!v.partial) return;
