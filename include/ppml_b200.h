@@ -158,13 +158,14 @@ int ppml_b200_repack_q8_0(const void* blocks34_dev, int64_t nblocks, void* q8_0r
  * A row of zeros has scale 0; a row that holds an infinity or a NaN has scale NaN and integers 0, so that its results are
  * NaN and no other row's are touched.  The sum is exact for every K up to PPML_B200_I8_MAX_K (beyond: status 9), whatever
  * the kernel; integers of -128 are fine.  Results are computed in fp32 and rounded once to c_type.  act as in
- * ppml_b200_mul_mat_f32_fused; bias (fp32) and gate (c_type) may be NULL.  Every matrix has a row pitch in elements (ld_*,
+ * ppml_b200_mul_mat_f32_fused (NaN stays NaN under each); bias (fp32) and gate (c_type) may be NULL.  Every matrix has a row pitch in elements (ld_*,
  * >= its row length; elements behind a row are neither read into results nor written).
  * quantize_tokens_i8 serves weights too: a row of W is an output channel.
  * path: AUTO / UMMA use the tensor cores where A and B are 16-byte aligned with pitches that are multiples of 16 bytes
  * (UMMA: status 7 otherwise), SIMT the CUDA cores; the sums are the same, so the results agree bit for bit for act = 0.
- * linear_i8 quantizes X on the way; at most four tokens (K up to 32768) run in one kernel on the CUDA cores (path UMMA: status 7)
- * and need no workspace.  workspace: device memory of ppml_b200_linear_i8_workspace(M, K) bytes, 16-byte aligned,
+ * The CUDA-core product takes N up to 4194240 (status 9).
+ * linear_i8 quantizes X on the way; at most four tokens (with K up to 32768) run in one kernel on the CUDA cores (path UMMA:
+ * status 7) and need no workspace.  workspace: device memory of ppml_b200_linear_i8_workspace(M, K) bytes, 16-byte aligned,
  * used on `stream` only while the call runs there.  M = 0 is a call without work (status 0). */
 #define PPML_B200_TYPE_F32 0
 #define PPML_B200_TYPE_F16 1

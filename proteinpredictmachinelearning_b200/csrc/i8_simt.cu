@@ -209,7 +209,7 @@ int launch_quantize_tokens(const void* x, int type, long long ld_x, int8_t* q, l
 
 int launch_i8_dp4a(const I8Product& p, cudaStream_t st) {
     const dim3 grid(static_cast<unsigned>((p.M + static_cast<long long>(kT) - 1) / kT), static_cast<unsigned>((p.N + static_cast<long long>(kT) - 1) / kT));
-    if (grid.y > 65535u) return ST_TOO_LARGE;
+    if ((p.N + static_cast<long long>(kT) - 1) / kT > 65535) return ST_TOO_LARGE;
     switch (p.c_type) {
         case kTypeF32: i8_dp4a_kernel<float><<<grid, 256, 0, st>>>(p); break;
         case kTypeF16: i8_dp4a_kernel<__half><<<grid, 256, 0, st>>>(p); break;

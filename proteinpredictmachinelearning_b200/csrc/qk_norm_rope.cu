@@ -216,7 +216,6 @@ __global__ void __launch_bounds__(32 * kWarps) qk_backward_kernel(const QkParams
     }
 }
 
-
 // ---- vector kernels ----------------------------------------------------------------------------------------------------
 // A lane holds two chunks of V neighbouring values (VB bytes each) that rotate with one another: chunks l and l + rot / 2 / V for
 // the pairs (i, i + rot / 2), chunks 2 l and 2 l + 1 for neighbouring pairs and for dims that pass.  So a rotation needs no
@@ -247,7 +246,6 @@ template <typename T> __device__ __forceinline__ uint64_t widen(uint32_t two) {
 }
 __device__ __forceinline__ uint32_t narrow2(float a, float b, __nv_bfloat16) { const __nv_bfloat162 t = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
 __device__ __forceinline__ uint32_t narrow2(float a, float b, __half) { const __half2 t = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
-__device__ __forceinline__ uint32_t narrow2(float a, float, float) { return __float_as_uint(a); }
 template <typename T, int VB> __device__ __forceinline__ void store_pairs(const uint64_t (&y)[VB / sizeof(T)], unsigned char* to, uint32_t a, uint32_t b, bool has_a, bool has_b) {
     constexpr int V = VB / sizeof(T), kWords = VB / 4;
     uint32_t w[2 * kWords];
@@ -269,8 +267,8 @@ template <typename T, int VB> __device__ __forceinline__ void store_pairs(const 
 // (n m) >> (32 + s) is exact; d = 1 has m = 0.
 __device__ __forceinline__ uint32_t div_by(uint32_t n, uint32_t m, int s) { return m == 0 ? n : __umulhi(n, m) >> s; }
 
-// 1 / sqrt(v): the hardware's estimate and one Newton step (within 1 unit in the last place; a division and a square root
-// take 40 instructions).  0 and infinity stay what the estimate makes of them.
+// 1 / sqrt(v): the hardware's estimate (2 units in the last place) and one Newton step, which leaves its rounding errors alone; a
+// division and a square root take 40 instructions.  0 and infinity stay what the estimate makes of them.
 __device__ __forceinline__ float inv_sqrt(float v) {
     const float r = rsqrtf(v);
     return r > 0.0f && r < __uint_as_float(0x7f800000u) ? fmaf(0.5f * r, fmaf(-v * r, r, 1.0f), r) : r;
@@ -561,6 +559,10 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
                     const uint64_t sgx2 = pack2(sgx, sgx), sg2 = pack2(sg, sg);
 #pragma unroll
                     for (int j = 0; j < V; ++j) y[j] = ffma2(ffma2(x[j], sgx2, y[j]), r2, sg2);
+                }
+                if (h + u >= live) {               // padding: 0 even under weights that are not finite
+#pragma unroll
+                    for (int j = 0; j < V; ++j) y[j] = 0;
                 }
                 if (h + u < count) store_pairs<T, VB>(y, m.dx, n.at_a, n.at_b, n.has_a, n.has_b);
                 m.dx += sd.dx.h;

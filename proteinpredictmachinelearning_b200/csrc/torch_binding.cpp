@@ -6,9 +6,12 @@
 // Wrong tensors raise ValueError, a status of the library RuntimeError; no C++ exception leaves a function.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
-#include <optional>
+#include <climits>
+#include <cstring>
+#include <stdexcept>
 #include <string>
 
 #include "../../include/ppml_b200.h"
@@ -72,8 +75,9 @@ int extent(int64_t n, const char* name) {
     if (n > INT_MAX) refuse(name, "an extent beyond 32 bits");
     return static_cast<int>(n);
 }
+// torch's CUDA allocation without its dispatcher (0.6 us less a tensor)
 at::Tensor fresh(at::IntArrayRef sizes, at::IntArrayRef strides, at::ScalarType type, c10::Device dev) {
-    return at::empty_strided(sizes, strides, at::TensorOptions().dtype(type).device(dev));
+    return at::Tensor(at::detail::empty_strided_cuda(sizes, strides, type, dev));
 }
 void* stream_of(c10::Device dev) { return at::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
@@ -233,7 +237,9 @@ struct QkArgs {
             cfg.pos_b = n == 2 ? p->stride(0) : 0;
             pos = static_cast<const int32_t*>(p->data_ptr());
         }
-        cfg.interleaved = PyObject_IsTrue(a[9]) == 1;
+        const int truth = PyObject_IsTrue(a[9]);
+        if (truth < 0) { PyErr_Clear(); refuse("interleaved", "a truth value is wanted"); }
+        cfg.interleaved = truth;
     }
 };
 // a new [B, L, h, d] like t, or the caller's own

@@ -517,7 +517,7 @@ cudaError_t launch_cluster(int grid, int cluster, size_t smem, cudaStream_t st, 
 }
 
 // How a product is cut: `pair` 1 persistent single CTAs, 2 persistent pairs, 0 one tile per cluster of `parts` CTAs.
-struct Plan { int pair, bn, parts; };
+struct Plan { int pair = 1, bn = 256, parts = 1; };
 
 // The cut with the shortest estimate, in cycles, for the busiest CTA.  A stage of 128 k takes 2.1 cycles a row (the rate at which
 // tiles come out of L2: a pair fetches half of the token rows each), a tile's epilogue 8 a token, a tile 400 besides, a pair's
@@ -525,9 +525,9 @@ struct Plan { int pair, bn, parts; };
 // against other cuts (us, bf16 results): 408 x 1024 -> 1024 32 tokens a tile 4.5, 128 in four parts 6.8; 200 x 8192 -> 1024 64 in four
 // parts 9.2, 32 in two 11.6; 1999 x 1000 -> 777 96 6.4, 128 6.9; 8192 x 256 -> 512 single 5.4, pairs 6.2; 5000 x 4000 -> 1000
 // pairs 24.4, single 30.6; 65536 x 256 -> 256 tiles of 256 13.5, of 128 14.5.
-Plan choose(const I8Product& p) {
+Plan choose_anew(const I8Product& p) {
     const long long sms = num_sms(), kb = (p.K + 127) / 128, M = p.M;
-    Plan best{1, 256, 1};
+    Plan best;
     long long least = INT64_MAX;
     auto consider = [&](Plan plan) {
         const int cg = plan.pair == 2 ? 2 : 1;
@@ -550,6 +550,16 @@ Plan choose(const I8Product& p) {
             for (int parts = 2; parts <= 8 && 2 * parts <= kb; parts *= 2) consider({0, most, parts});
     }
     return best;
+}
+
+// The choice follows from the sizes alone; a thread keeps the last ones (the search takes 1 us).
+Plan choose(const I8Product& p) {
+    struct Kept { int M = 0, K = 0, N = 0, sms = 0; Plan plan; };
+    static thread_local Kept kept[16];
+    const int sms = num_sms();
+    Kept& k = kept[(static_cast<unsigned>(p.M) * 31u + static_cast<unsigned>(p.K) * 7u + static_cast<unsigned>(p.N)) >> 3 & 15u];
+    if (k.M != p.M || k.K != p.K || k.N != p.N || k.sms != sms) k = Kept{p.M, p.K, p.N, sms, choose_anew(p)};
+    return k.plan;
 }
 
 template <typename T, int MORE>

@@ -343,6 +343,7 @@ def test_bad_arguments_are_refused_on_the_host(lib):
                 dict(C=C.c_void_p(66)), dict(C=C.c_void_p(65), c_type=1), dict(bias=C.c_void_p(66)), dict(a_scale=C.c_void_p(65))):
         assert mm(**bad) == 1, bad
     assert mm(K=131072, lda=1 << 18, ldb=1 << 18) == 9
+    assert mm(N=4194241, ldc=4194241, path=1) == 9
     assert mm(M=0) == 0 and mm(M=0, A=None, C=None, a_scale=None) == 0
     assert mm(path=2, A=C.c_void_p(68)) == 7 and mm(path=2, lda=17) == 7 and mm(path=2, B=C.c_void_p(72)) == 7 and mm(path=2, ldb=24) == 7
 
@@ -372,6 +373,7 @@ def test_wrong_tensors_are_refused():
                 lambda: ops.mul_mat_i8(q, s, W, ws, act="swish"), lambda: ops.mul_mat_i8(q, s, W, ws, dtype=torch.float64),
                 lambda: ops.mul_mat_i8(q, s, W, ws, out=torch.zeros((8, 4), device="cuda").t()),
                 lambda: ops.mul_mat_i8(q, s, W, ws, out=torch.zeros((1, 8), device="cuda").expand(4, 8)),
+                lambda: ops.linear_i8(x, W, None), lambda: ops.linear_i8(x, W, ws, path="auto"), lambda: ops.linear_i8(x, W, ws, dtype="bf16"),
                 lambda: ops.linear_i8(x, W[:, ::2], ws), lambda: ops.linear_i8(x[:, ::2], W[:, :16], ws), lambda: ops.linear_i8(x, W, ws, dtype=torch.int8)):
         with pytest.raises(ValueError):
             bad()

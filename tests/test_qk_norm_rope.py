@@ -273,6 +273,9 @@ def test_positions_padding_and_the_end_of_the_table(d, dtype, no_device_abort):
         c64, s64 = table_rows(cos, sin, pos, B, L)
         c64, s64 = c64[keep][None], s64[keep][None]
         check_backward(dx[keep][None], g[name], x[keep][None], dy[keep][None], w, "rms", 1e-6, c64, s64, False)
+    bad = torch.full((d,), float("nan"), device="cuda")
+    g = ops.qk_norm_rope_backward(q2, k2, dq, dk, bad, bad, cos=cos, sin=sin, positions=pad)
+    assert not g["dQ"][~keep].any() and not g["dK"][~keep].any()      # whatever the weights are
     far = pos.clone()
     far[1, 3], far[2, 20] = rows, 2147483647
     ok = (far >= 0) & (far < rows)
@@ -541,7 +544,8 @@ def test_wrong_tensors_are_refused():
                 lambda: ops.qk_norm_rope(q, k, q_weight=w[:8]), lambda: ops.qk_norm_rope(q, k, q_weight=w.half()), lambda: ops.qk_norm_rope(q, k, cos=cos),
                 lambda: ops.qk_norm_rope(q, k, cos=cos, sin=sin[:, :4]), lambda: ops.qk_norm_rope(q, k, cos=cos.double(), sin=sin.double()),
                 lambda: ops.qk_norm_rope(q, k, cos=cos, sin=sin, positions=pos.long()), lambda: ops.qk_norm_rope(q, k, cos=cos, sin=sin, positions=pos[:, :4]),
-                lambda: ops.qk_norm_rope(q, k, cos=cos.cpu(), sin=sin.cpu()), lambda: ops.qk_norm_rope(q, k, eps="1"),
+                lambda: ops.qk_norm_rope(q, k, cos=cos.cpu(), sin=sin.cpu()), lambda: ops.qk_norm_rope(q, k, eps="1"), lambda: ops.qk_norm_rope(q, k, interleaved=q),
+                lambda: ops.qk_norm_rope(q, [k]),
                 lambda: ops.qk_norm_rope(q, None, out=(q, k)), lambda: ops.qk_norm_rope(q, k, out=(q, q)), lambda: ops.qk_norm_rope(q, k, out=(q.half(), k)),
                 lambda: ops.qk_norm_rope_backward(q, k, q, None), lambda: ops.qk_norm_rope_backward(q, k, q, k[:, :3])):
         with pytest.raises(ValueError):
