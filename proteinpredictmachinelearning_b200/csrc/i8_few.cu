@@ -4,6 +4,7 @@
 // into shared memory while its first weights are on their way, instead of a kernel of its own doing it first.  A warp
 // takes R output channels and sums them with dp4a against all tokens: 4 multiply-adds an instruction cover up to kI8Few tokens at
 // the memory's rate.  16 bytes of a weight row per lane and step; the integers of the tokens come from shared memory.
+// Latency-bound: 1 x 1024 -> 4096 bf16 3.2 us from launch to launch, against 6.3 of the two kernels it replaces.
 #include "i8_common.cuh"
 
 namespace ppml_b200 {
