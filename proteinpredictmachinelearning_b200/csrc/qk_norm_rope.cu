@@ -246,23 +246,6 @@ template <typename T> __device__ __forceinline__ uint64_t widen(uint32_t two) {
 }
 __device__ __forceinline__ uint32_t narrow2(float a, float b, __nv_bfloat16) { const __nv_bfloat162 t = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
 __device__ __forceinline__ uint32_t narrow2(float a, float b, __half) { const __half2 t = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
-template <typename T, int VB> __device__ __forceinline__ void store_pairs(const uint64_t (&y)[VB / sizeof(T)], unsigned char* to, uint32_t a, uint32_t b, bool has_a, bool has_b) {
-    constexpr int V = VB / sizeof(T), kWords = VB / 4;
-    uint32_t w[2 * kWords];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        float lo, hi;
-        unpack2(y[j], lo, hi);
-        if constexpr (sizeof(T) == 2) w[j] = narrow2(lo, hi, T());
-        else { w[2 * j] = __float_as_uint(lo); w[2 * j + 1] = __float_as_uint(hi); }
-    }
-    typename RawOf<VB>::type ra, rb;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) { reinterpret_cast<uint32_t*>(&ra)[i] = w[i]; reinterpret_cast<uint32_t*>(&rb)[i] = w[kWords + i]; }
-    if (has_a) *reinterpret_cast<typename RawOf<VB>::type*>(to + a) = ra;
-    if (has_b) *reinterpret_cast<typename RawOf<VB>::type*>(to + b) = rb;
-}
-
 // n / d for n < 2^31: with 2^s < d <= 2^(s + 1) and m = ceil(2^(32 + s) / d) the error m d - 2^(32 + s) is below 2^(s + 1), so that
 // (n m) >> (32 + s) is exact; d = 1 has m = 0.
 __device__ __forceinline__ uint32_t div_by(uint32_t n, uint32_t m, int s) { return m == 0 ? n : __umulhi(n, m) >> s; }
@@ -309,10 +292,11 @@ template <int V> __device__ __forceinline__ void load_table(const QkVec& v, cons
             if (i < n.turning) { c[i] = v.cos_t[at + i]; s[i] = v.sin_t[at + i]; }     // neighbours: may end inside the chunk
     }
 }
-__device__ __forceinline__ float group_sum(float v, int G) {
+// Sum over the lanes of a row; LG >= 0: their number is 2^LG, else G (a branch per step).
+template <int LG> __device__ __forceinline__ float group_sum(float v, int G) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
-        if (o < G) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (LG >= 0 ? o < (1 << (LG >= 0 ? LG : 0)) : o < G) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 template <int N> __device__ __forceinline__ float lane_sum(const uint64_t (&x)[N]) {
@@ -330,10 +314,10 @@ template <int N> __device__ __forceinline__ float lane_dot(const uint64_t (&x)[N
     return a + b;
 }
 // x becomes x - mean; returns 1 / sqrt(..) of the row.  Values that do not exist stay 0.
-template <int V> __device__ __forceinline__ float normalizer(const QkVec& v, const Lane& n, float inv_d, uint64_t (&x)[V]) {
+template <int V, int LG> __device__ __forceinline__ float normalizer(const QkVec& v, const Lane& n, float inv_d, uint64_t (&x)[V]) {
     if (v.norm == 0) return 1.0f;
     if (v.norm == 2) {
-        const float m = group_sum(lane_sum(x), v.G) * inv_d;
+        const float m = group_sum<LG>(lane_sum(x), v.G) * inv_d;
         const uint64_t m2 = pack2(-m, -m);
 #pragma unroll
         for (int j = 0; j < V; ++j) x[j] = fadd2(x[j], m2);
@@ -345,7 +329,7 @@ template <int V> __device__ __forceinline__ float normalizer(const QkVec& v, con
             }
         }
     }
-    return inv_sqrt(fmaf(group_sum(lane_dot(x, x), v.G), inv_d, v.eps));
+    return inv_sqrt(fmaf(group_sum<LG>(lane_dot(x, x), v.G), inv_d, v.eps));
 }
 __device__ __forceinline__ uint64_t swap2(uint64_t p) { float a, b; unpack2(p, a, b); return pack2(b, a); }
 // y = x * c + partner * s.  The partner of a packed pair is the same place of the other chunk, or with neighbouring pairs (and with
@@ -353,19 +337,23 @@ __device__ __forceinline__ uint64_t swap2(uint64_t p) { float a, b; unpack2(p, a
 // times 0.
 template <int V> __device__ __forceinline__ void turn(const QkVec& v, const Lane& n, const uint64_t (&x)[V], const uint64_t (&c)[V], const uint64_t (&s)[V],
                                                       uint64_t (&y)[V]) {
-    if (V == 1 || v.interleaved) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            y[j] = fmul2(x[j], c[j]);
-            if (v.all_turn || j < n.turning) y[j] = ffma2(swap2(x[j]), s[j], y[j]);
-        }
-    } else {
+    for (int j = 0; j < V; ++j) y[j] = fmul2(x[j], c[j]);
+    if (v.all_turn) {
+        if (V == 1 || v.interleaved) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) y[j] = fmul2(x[j], c[j]);
-        if (v.all_turn || n.turning) {
+            for (int j = 0; j < V; ++j) y[j] = ffma2(swap2(x[j]), s[j], y[j]);
+        } else {
 #pragma unroll
             for (int j = 0; j < V; ++j) y[j] = ffma2(x[(j + V / 2) % V], s[j], y[j]);
         }
+    } else if (V == 1 || v.interleaved) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < n.turning) y[j] = ffma2(swap2(x[j]), s[j], y[j]);
+    } else if (n.turning) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[j] = ffma2(x[(j + V / 2) % V], s[j], y[j]);
     }
 }
 // The factors of turn() from the lane's cos and sin and the weights of its values.
@@ -391,15 +379,12 @@ template <int V> __device__ __forceinline__ void factors(const QkVec& v, const L
 }
 // Turns a gradient back, in place, from the lane's cos and sin alone (half the registers of factors()).
 template <int V> __device__ __forceinline__ void turn_back(const QkVec& v, const Lane& n, const float (&c)[V], const float (&s)[V], uint64_t (&y)[V]) {
-    if (V == 1 || v.interleaved) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if (!(v.all_turn || j < n.turning)) continue;
-            float a, b;
-            unpack2(y[j], a, b);
-            y[j] = pack2(fmaf(b, s[j], a * c[j]), fmaf(-a, s[j], b * c[j]));
-        }
-    } else if (v.all_turn || n.turning) {
+    auto neighbours = [&](int j) {
+        float a, b;
+        unpack2(y[j], a, b);
+        y[j] = pack2(fmaf(b, s[j], a * c[j]), fmaf(-a, s[j], b * c[j]));
+    };
+    auto halves = [&]() {
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) {
             const uint64_t c2 = pack2(c[2 * j], c[2 * j + 1]), s2 = pack2(s[2 * j], s[2 * j + 1]), a = y[j], b = y[V / 2 + j];
@@ -407,6 +392,20 @@ template <int V> __device__ __forceinline__ void turn_back(const QkVec& v, const
             y[j] = ffma2(b, s2, fmul2(a, c2));
             y[V / 2 + j] = ffma2(a, minus, fmul2(b, c2));
         }
+    };
+    if (v.all_turn) {
+        if (V == 1 || v.interleaved) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) neighbours(j);
+        } else {
+            halves();
+        }
+    } else if (V == 1 || v.interleaved) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < n.turning) neighbours(j);
+    } else if (n.turning) {
+        halves();
     }
 }
 
@@ -442,13 +441,46 @@ template <typename T, int VB> __device__ __forceinline__ void pairs_of(const typ
         else x[j] = pack2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
     }
 }
+// Predicated accesses: a row's two dozen conditions would be branches otherwise.
 template <int VB> __device__ __forceinline__ typename RawOf<VB>::type load_raw(const unsigned char* p, bool yes) {
-    using Raw = typename RawOf<VB>::type;
-    return yes ? *reinterpret_cast<const Raw*>(p) : Raw{};
+    typename RawOf<VB>::type r;
+    const int on = yes;
+    if constexpr (VB == 16)
+        asm volatile("{.reg .pred p; setp.ne.s32 p, %5, 0; mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; mov.b32 %3, 0; "
+                     "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];}" : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w) : "l"(p), "r"(on) : "memory");
+    else if constexpr (VB == 8)
+        asm volatile("{.reg .pred p; setp.ne.s32 p, %3, 0; mov.b32 %0, 0; mov.b32 %1, 0; @p ld.global.v2.b32 {%0, %1}, [%2];}"
+                     : "=&r"(r.x), "=&r"(r.y) : "l"(p), "r"(on) : "memory");
+    else asm volatile("{.reg .pred p; setp.ne.s32 p, %2, 0; mov.b32 %0, 0; @p ld.global.b32 %0, [%1];}" : "=&r"(r) : "l"(p), "r"(on) : "memory");
+    return r;
+}
+template <int VB> __device__ __forceinline__ void store_raw(unsigned char* p, const typename RawOf<VB>::type& r, bool yes) {
+    const int on = yes;
+    if constexpr (VB == 16)
+        asm volatile("{.reg .pred p; setp.ne.s32 p, %5, 0; @p st.global.v4.b32 [%4], {%0, %1, %2, %3};}" ::"r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "l"(p), "r"(on) : "memory");
+    else if constexpr (VB == 8)
+        asm volatile("{.reg .pred p; setp.ne.s32 p, %3, 0; @p st.global.v2.b32 [%2], {%0, %1};}" ::"r"(r.x), "r"(r.y), "l"(p), "r"(on) : "memory");
+    else asm volatile("{.reg .pred p; setp.ne.s32 p, %2, 0; @p st.global.b32 [%1], %0;}" ::"r"(r), "l"(p), "r"(on) : "memory");
+}
+template <typename T, int VB> __device__ __forceinline__ void store_pairs(const uint64_t (&y)[VB / sizeof(T)], unsigned char* to, uint32_t a, uint32_t b, bool has_a, bool has_b) {
+    constexpr int V = VB / sizeof(T), kWords = VB / 4;
+    uint32_t w[2 * kWords];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float lo, hi;
+        unpack2(y[j], lo, hi);
+        if constexpr (sizeof(T) == 2) w[j] = narrow2(lo, hi, T());
+        else { w[2 * j] = __float_as_uint(lo); w[2 * j + 1] = __float_as_uint(hi); }
+    }
+    typename RawOf<VB>::type ra, rb;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) { reinterpret_cast<uint32_t*>(&ra)[i] = w[i]; reinterpret_cast<uint32_t*>(&rb)[i] = w[kWords + i]; }
+    store_raw<VB>(to + a, ra, has_a);
+    store_raw<VB>(to + b, rb, has_b);
 }
 
 // U rows of every group of lanes are requested together.
-template <typename T, int VB, int U, int BLOCKS>
+template <typename T, int VB, int U, int BLOCKS, int LG>
 __global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const __grid_constant__ QkVec v) {
     constexpr int V = VB / sizeof(T);
     using Raw = typename RawOf<VB>::type;
@@ -483,12 +515,12 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const __gri
             for (int u = 0; u < U; ++u) {
                 uint64_t x[V], y[V];
                 pairs_of<T, VB>(ra[u], rb[u], x);
-                const float rs = normalizer<V>(v, n, inv_d, x);
+                const float rs = normalizer<V, LG>(v, n, inv_d, x);
                 const uint64_t r2 = pack2(rs, rs);
 #pragma unroll
                 for (int j = 0; j < V; ++j) x[j] = fmul2(x[j], r2);
                 turn<V>(v, n, x, c, s, y);
-                if (h + u < count) store_pairs<T, VB>(y, m.y, n.at_a, n.at_b, n.has_a, n.has_b);
+                store_pairs<T, VB>(y, m.y, n.at_a, n.at_b, n.has_a && h + u < count, n.has_b && h + u < count);
                 m.y += sd.y.h;
             }
             h += U;
@@ -498,7 +530,7 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const __gri
     }
 }
 
-template <typename T, int VB, int U, int BLOCKS>
+template <typename T, int VB, int U, int BLOCKS, int LG>
 __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __grid_constant__ QkVec v) {
     constexpr int V = VB / sizeof(T);
     using Raw = typename RawOf<VB>::type;
@@ -542,7 +574,7 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
                 pairs_of<T, VB>(ga[u], gb[u], y);
                 turn_back<V>(v, n, c, s, y);
                 __syncwarp();
-                float rs = normalizer<V>(v, n, inv_d, x);
+                float rs = normalizer<V, LG>(v, n, inv_d, x);
                 if (h + u >= live) rs = 0.0f;      // a row of zeros then: with eps = 0 its xhat would be NaN
                 const uint64_t r2 = pack2(rs, rs);
 #pragma unroll
@@ -554,8 +586,8 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
                     y[j] = fmul2(y[j], pack2(w0, w1));
                 }
                 if (v.norm != 0) {
-                    const float sgx = -group_sum(lane_dot(y, x), v.G) * inv_d;
-                    const float sg = v.norm == 2 ? -rs * group_sum(lane_sum(y), v.G) * inv_d : 0.0f;
+                    const float sgx = -group_sum<LG>(lane_dot(y, x), v.G) * inv_d;
+                    const float sg = v.norm == 2 ? -rs * group_sum<LG>(lane_sum(y), v.G) * inv_d : 0.0f;
                     const uint64_t sgx2 = pack2(sgx, sgx), sg2 = pack2(sg, sg);
 #pragma unroll
                     for (int j = 0; j < V; ++j) y[j] = ffma2(ffma2(x[j], sgx2, y[j]), r2, sg2);
@@ -564,7 +596,7 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
 #pragma unroll
                     for (int j = 0; j < V; ++j) y[j] = 0;
                 }
-                if (h + u < count) store_pairs<T, VB>(y, m.dx, n.at_a, n.at_b, n.has_a, n.has_b);
+                store_pairs<T, VB>(y, m.dx, n.at_a, n.at_b, n.has_a && h + u < count, n.has_b && h + u < count);
                 m.dx += sd.dx.h;
             }
             h += U;
@@ -670,9 +702,27 @@ cudaError_t launch_vec(const QkParams& p, QkVec& v, bool backward, cudaStream_t 
     }
     v.side[0].blocks = static_cast<uint32_t>(bq); v.side[1].blocks = static_cast<uint32_t>(bk);
     const dim3 grid(static_cast<unsigned>(bq + bk));
-    // rows at once and blocks an SM: as many as the registers hold without spilling
-    if (!backward) return launch_pdl(qk_vec_forward_kernel<T, VB, kHeadsAtOnce, V == 8 ? 2 : V == 4 ? 3 : 4>, grid, dim3(256), 0, st, v);
-    cudaError_t e = launch_pdl(qk_vec_backward_kernel<T, VB, V == 8 ? 2 : 4, 2>, grid, dim3(256), v.partial ? 8u * p.d * sizeof(float) : 0u, st, v);
+    // rows at once and blocks an SM: as many as the registers hold without spilling; the lanes of a row are known to the instances
+    // with 16-byte chunks
+    constexpr int kForward = V == 8 ? 2 : V == 4 ? 3 : 4, kBackwardRows = V == 8 ? 2 : 4;
+    const size_t lines = v.partial ? 8u * p.d * sizeof(float) : 0u;
+    cudaError_t e;
+#define PPML_LG(LG) e = backward ? launch_pdl(qk_vec_backward_kernel<T, VB, kBackwardRows, 2, LG>, grid, dim3(256), lines, st, v) \
+                                 : launch_pdl(qk_vec_forward_kernel<T, VB, kHeadsAtOnce, kForward, LG>, grid, dim3(256), 0, st, v)
+    if constexpr (VB == 16) {
+        switch (v.G) {
+            case 1: PPML_LG(0); break;
+            case 2: PPML_LG(1); break;
+            case 4: PPML_LG(2); break;
+            case 8: PPML_LG(3); break;
+            case 16: PPML_LG(4); break;
+            default: PPML_LG(5);
+        }
+    } else {
+        PPML_LG(-1);
+    }
+#undef PPML_LG
+    if (!backward) return e;
     if (e == cudaSuccess && v.partial)
         e = launch_pdl(qk_weight_sum_kernel, dim3((p.d + 31) / 32, 2), dim3(1024), 0, st, static_cast<const float*>(v.partial), static_cast<int>(bq),
                        static_cast<int>(bk), p.d, p.dqw, p.dkw);
