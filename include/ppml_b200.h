@@ -164,8 +164,9 @@ int ppml_b200_repack_q8_0(const void* blocks34_dev, int64_t nblocks, void* q8_0r
  * path: AUTO / UMMA use the tensor cores where A and B are 16-byte aligned with pitches that are multiples of 16 bytes
  * (UMMA: status 7 otherwise), SIMT the CUDA cores; the sums are the same, so the results agree bit for bit for act = 0.
  * The CUDA-core product takes N up to 4194240 (status 9).
- * linear_i8 quantizes X on the way; at most four tokens (with K up to 32768) run in one kernel on the CUDA cores (path UMMA:
- * status 7) and need no workspace.  workspace: device memory of ppml_b200_linear_i8_workspace(M, K) bytes, 16-byte aligned,
+ * linear_i8 quantizes X on the way; one to four tokens of a short K (up to 8192, 4096 for two tokens, 2048 for three and four) run in
+ * one kernel on the CUDA cores (path UMMA: status 7) and need no workspace (ppml_b200_linear_i8_workspace gives 0).  C shares no
+ * element with X; gate may be C.  workspace: device memory of ppml_b200_linear_i8_workspace(M, K) bytes, 16-byte aligned,
  * used on `stream` only while the call runs there.  M = 0 is a call without work (status 0). */
 #define PPML_B200_TYPE_F32 0
 #define PPML_B200_TYPE_F16 1

@@ -108,23 +108,23 @@ __global__ void __launch_bounds__(kFewThreads) i8_few_kernel(const TX* __restric
 
 template <typename TX, typename TC, int MT, int R>
 cudaError_t launch_r(const TX* x, long long ld_x, const I8Product& p, cudaStream_t st) {
-    auto kernel = i8_few_kernel<TX, TC, MT, R>;
-    const size_t smem = static_cast<size_t>(MT) * ((p.K + 15) / 16 * 16);
-    if (smem > 40 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kI8FewBytes);
-        if (e != cudaSuccess) return e;
-    }
     const long long per = kFewWarps * R;
-    return launch_pdl(kernel, dim3(static_cast<unsigned>((p.N + per - 1) / per)), dim3(kFewThreads), smem, st, x, ld_x, p);
+    return launch_pdl(i8_few_kernel<TX, TC, MT, R>, dim3(static_cast<unsigned>((p.N + per - 1) / per)), dim3(kFewThreads),
+                      static_cast<size_t>(MT) * ((p.K + 15) / 16 * 16), st, x, ld_x, p);
+}
+template <typename TX, typename TC, int MT>
+cudaError_t launch_m(const TX* x, long long ld_x, const I8Product& p, cudaStream_t st) {
+    // About two blocks an SM: every block quantizes the tokens again, and every warp should have its weights on the way at once.
+    // Measured with 1 and with 4 channels a warp: 1 x 1024 -> 1024 2.5 and 3.2 us, 3 x 2048 -> 2048 4.6 and 6.7, 1 x 4096 -> 8192
+    // 14.6 and 10.4.
+    const long long blocks = 2ll * num_sms();
+    if (p.N <= kFewWarps * blocks) return launch_r<TX, TC, MT, 1>(x, ld_x, p, st);
+    if (p.N <= 2 * kFewWarps * blocks) return launch_r<TX, TC, MT, 2>(x, ld_x, p, st);
+    return launch_r<TX, TC, MT, 4>(x, ld_x, p, st);
 }
 template <typename TX, typename TC>
 int launch_x(const TX* x, long long ld_x, const I8Product& p, cudaStream_t st) {
-    // four channels per warp where that still gives most SMs a block, else one
-    const bool four = p.N >= 32 * 96;
-    cudaError_t e;
-    if (p.M == 1) e = four ? launch_r<TX, TC, 1, 4>(x, ld_x, p, st) : launch_r<TX, TC, 1, 1>(x, ld_x, p, st);
-    else if (p.M == 2) e = four ? launch_r<TX, TC, 2, 4>(x, ld_x, p, st) : launch_r<TX, TC, 2, 1>(x, ld_x, p, st);
-    else e = four ? launch_r<TX, TC, 4, 4>(x, ld_x, p, st) : launch_r<TX, TC, 4, 1>(x, ld_x, p, st);
+    const cudaError_t e = p.M == 1 ? launch_m<TX, TC, 1>(x, ld_x, p, st) : p.M == 2 ? launch_m<TX, TC, 2>(x, ld_x, p, st) : launch_m<TX, TC, 4>(x, ld_x, p, st);
     if (e != cudaSuccess) { cudaGetLastError(); return ST_LAUNCH; }
     return ST_OK;
 }
@@ -136,7 +136,9 @@ int launch_c(const TX* x, long long ld_x, const I8Product& p, cudaStream_t st) {
 
 }  // namespace
 
-bool i8_few(long long M, int K) { return M <= kI8Few && (M <= 2 ? M : 4) * ((K + 15ll) / 16 * 16) <= kI8FewBytes; }
+// Up to four tokens, as long as quantizing them in every block costs less than a kernel before the product: 2 x 4096 -> 8192 takes
+// 11.5 us this way and 11.2 in two kernels, 1 x 4096 -> 8192 10.4 and 11.1, 4 x 8192 -> 1024 15 and 8.
+bool i8_few(long long M, int K) { return M <= kI8Few && (M <= 2 ? M : 4) * ((K + 15ll) / 16 * 16) <= kI8FewValues; }
 
 int launch_i8_few(const void* x, int x_type, long long ld_x, const I8Product& p, cudaStream_t st) {
     switch (x_type) {

@@ -135,7 +135,7 @@ int launch_quantize_tokens(const void* x, int type, long long ld_x, int8_t* q, l
                            cudaStream_t st);
 int launch_i8_dp4a(const I8Product& p, cudaStream_t st);
 // quantizer and product in one kernel for at most kI8Few tokens (i8_few.cu); p.A, p.lda and p.a_scale are not used
-constexpr int kI8Few = 4, kI8FewBytes = 128 * 1024;      // of tokens, and of their integers in shared memory
+constexpr int kI8Few = 4, kI8FewValues = 8192;           // tokens, and their values together
 bool i8_few(long long M, int K);
 int launch_i8_few(const void* x, int x_type, long long ld_x, const I8Product& p, cudaStream_t st);
 // tcgen05 (umma_i8.cu): 16-byte aligned operands and pitches, ST_UNSUPPORTED_PATH otherwise

@@ -227,7 +227,7 @@ def test_largest_sums_are_exact(M, N, no_device_abort):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_linear_is_quantizer_and_product(M, dtype, no_device_abort):
     """One call, two calls, the CUDA-core path and any part of the tokens give the same bits."""
-    for K, N in ((272, 200), (100, 64), (2049, 72), (528, 3500), (5000, 9), (34000, 24)):
+    for K, N in ((272, 200), (100, 64), (2049, 72), (528, 3500), (144, 9000), (5000, 9), (8192, 24), (8193, 24)):
         x = rows(M, K, dtype, M, K + 8)
         W, ws = ops.quantize_tokens_i8(rows(N, K, F32, 9) * 0.02)
         bias = scales(N, 5)
@@ -243,6 +243,19 @@ def test_linear_is_quantizer_and_product(M, dtype, no_device_abort):
     y = ops.linear_i8(x, W, scales(90, 2), gate=gate, act="gelu", dtype=F32)
     q, s = ops.quantize_tokens_i8(x)
     check_product(y, q, s, W, scales(90, 2), None, gate, "gelu")
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N", [(2, 272, 200), (30, 2048, 136), (300, 272, 264), (9000, 80, 300)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gate_may_be_the_output(M, K, N, dtype, no_device_abort):
+    x, gate = rows(M, K, dtype, 1), rows(M, N, dtype, 2)
+    W, ws = ops.quantize_tokens_i8(rows(N, K, F32, 3) * 0.02)
+    for path in (PATH_AUTO, PATH_SIMT):
+        want = ops.linear_i8(x, W, ws, gate=gate, act="silu", path=path)
+        own = gate.clone()
+        ops.linear_i8(x, W, ws, gate=own, act="silu", out=own, path=path)
+        assert torch.equal(own, want)
 
 
 @gpu
@@ -348,7 +361,8 @@ def test_bad_arguments_are_refused_on_the_host(lib):
     assert mm(path=2, A=C.c_void_p(68)) == 7 and mm(path=2, lda=17) == 7 and mm(path=2, B=C.c_void_p(72)) == 7 and mm(path=2, ldb=24) == 7
 
     assert lib.ppml_b200_linear_i8_workspace(5, 17) == 5 * 32 + 32 and lib.ppml_b200_linear_i8_workspace(0, 17) == 0
-    assert lib.ppml_b200_linear_i8_workspace(4, 17) == 0 and lib.ppml_b200_linear_i8_workspace(4, 32769) == 4 * 32784 + 16
+    assert lib.ppml_b200_linear_i8_workspace(4, 2048) == 0 and lib.ppml_b200_linear_i8_workspace(4, 2049) == 4 * 2064 + 16
+    assert lib.ppml_b200_linear_i8_workspace(1, 8192) == 0 and lib.ppml_b200_linear_i8_workspace(2, 4097) == 2 * 4112 + 16
     names = ("X", "x_type", "ld_x", "B", "ldb", "b_scale", "C", "ldc", "c_type", "M", "K", "N", "bias", "gate", "ld_gate", "act", "path", "ws", "bytes")
     good = (p, 0, 16, p, 16, p, p, 8, 0, 6, 16, 8, None, None, 0, 0, 0, p, 128)
 
