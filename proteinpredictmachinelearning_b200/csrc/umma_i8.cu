@@ -526,20 +526,25 @@ struct Plan { int pair = 1, bn = 256, parts = 1; };
 
 // The cut with the shortest estimate, in cycles, for the busiest CTA.  A stage of 128 k takes 2.1 cycles a row (the rate at which
 // tiles come out of L2: a pair fetches half of the token rows each), a tile's epilogue 8 a token, a tile 400 besides, a pair's
-// hand-shakes 800; parts of K cost 1600 + 49 a token for the partial sums' way through shared memory.  Fitted to the following, best
+// hand-shakes 800; parts of K cost 1300 + 30 a token for the partial sums' way through shared memory, and a B200 holds at once only as
+// many clusters of 2, 4 and 8 CTAs as kClustersHeld says.  Over 70 sizes of 1 to 8192 tokens the cut so chosen is 1.2 % slower than the
+// fastest one in the mean (17 % at most); without kClustersHeld it was 84 % at 1 x 4096 -> 2048 (9.7 for 5.3 us).  Best
 // against other cuts (us, bf16 results): 408 x 1024 -> 1024 32 tokens a tile 4.5, 128 in four parts 6.8; 200 x 8192 -> 1024 64 in four
 // parts 9.2, 32 in two 11.6; 1999 x 1000 -> 777 96 6.4, 128 6.9; 8192 x 256 -> 512 single 5.4, pairs 6.2; 5000 x 4000 -> 1000
 // pairs 24.4, single 30.6; 65536 x 256 -> 256 tiles of 256 13.5, of 128 14.5.
+constexpr int kClustersHeld[9] = {0, 148, 74, 0, 33, 0, 0, 0, 15};     // one CTA an SM, cudaOccupancyMaxActiveClusters
+
 Plan choose_anew(const I8Product& p) {
     const long long sms = num_sms(), kb = (p.K + 127) / 128, M = p.M;
     Plan best;
     long long least = INT64_MAX;
     auto consider = [&](Plan plan) {
         const int cg = plan.pair == 2 ? 2 : 1;
-        const long long tn = (p.N + 128ll * cg - 1) / (128 * cg), tt = (M + plan.bn - 1) / plan.bn, units = tn * tt * plan.parts;
-        const long long rounds = (units + sms / cg - 1) / (sms / cg), steps = (kb + plan.parts - 1) / plan.parts;
+        const long long tn = (p.N + 128ll * cg - 1) / (128 * cg), tt = (M + plan.bn - 1) / plan.bn, units = tn * tt;
+        const long long at_once = plan.pair == 0 ? kClustersHeld[plan.parts] : sms / cg;
+        const long long rounds = (units + at_once - 1) / at_once, steps = (kb + plan.parts - 1) / plan.parts;
         const long long fill = steps * (128 + plan.bn / cg) * 21 / 10;
-        const long long cost = rounds * (fill + (plan.pair == 0 ? 1600 + 49 * plan.bn : 8 * plan.bn + 400 + (cg == 2 ? 800 : 0)));
+        const long long cost = rounds * (fill + (plan.pair == 0 ? 1300 + 30 * plan.bn : 8 * plan.bn + 400 + (cg == 2 ? 800 : 0)));
         if (cost < least) { least = cost; best = plan; }
     };
     const int most = M >= 256 ? 256 : static_cast<int>((M + 15) / 16 * 16);        // whole tiles of tokens for small M
