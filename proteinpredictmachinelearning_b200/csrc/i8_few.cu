@@ -3,8 +3,11 @@
 // The weights are the traffic (N K bytes, each read once); a token's row is small, so every block quantizes all tokens for itself
 // into shared memory while its first weights are on their way, instead of a kernel of its own doing it first.  A warp
 // takes R output channels and sums them with dp4a against all tokens: 4 multiply-adds an instruction cover up to kI8Few tokens at
-// the memory's rate.  16 bytes of a weight row per lane and step; the integers of the tokens come from shared memory.
-// Latency-bound: 1 x 1024 -> 4096 bf16 3.2 us from launch to launch, against 6.3 of the two kernels it replaces.
+// the memory's rate.  16 bytes of a weight row per lane and step, kDeep steps of them on the way before the tokens are quantized;
+// the integers of the tokens come from shared memory.  Each sum ends in a lane of its own, so that the scales are fetched and the
+// results finished all at once (one after the other, 4 x 512 -> 8192 took 6.5 us for 3.8).
+// Latency-bound: 1 x 1024 -> 4096 bf16 2.5 us from launch to launch, against 5.4 of the two kernels it replaces; 1 x 4096 -> 8192
+// 9.0 us, 3.7 TB/s of weights.
 #include "i8_common.cuh"
 
 namespace ppml_b200 {
@@ -12,13 +15,8 @@ namespace {
 
 constexpr int kFewThreads = 256, kFewWarps = 8;
 
-__device__ __forceinline__ uint4 load16(const int8_t* row, int k, int K, bool vec) {
-    if (vec && k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (k + i < K) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i & 3));
-    return make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ uint4 load16(const int8_t* row, int k, int k_vec) {
+    return k < k_vec ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
     acc = __dp4a(static_cast<int>(a.x), static_cast<int>(b.x), acc);
@@ -29,22 +27,30 @@ __device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int acc) {
 
 template <typename TX, typename TC, int MT, int R>
 __global__ void __launch_bounds__(kFewThreads) i8_few_kernel(const TX* __restrict__ x, long long ld_x, const I8Product p) {
-    constexpr int N = Vec16<TX>::kN, kPer = kFewThreads / MT, kWarpsPer = kPer / 32;
+    constexpr int N = Vec16<TX>::kN, kPer = kFewThreads / MT, kWarpsPer = kPer / 32, kDeep = R == 1 ? 4 : 2;
     extern __shared__ __align__(16) int8_t xq[];   // [MT][K16]
     __shared__ uint32_t part[kFewWarps];
     __shared__ float scales[MT];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int k16 = (p.K + 15) & ~15;
     const long long n0 = (static_cast<long long>(blockIdx.x) * kFewWarps + warp) * R;
-    const bool w_vec = ((reinterpret_cast<uintptr_t>(p.B) | static_cast<uintptr_t>(p.ldb)) & 15) == 0;
+    const int kw_vec = ((reinterpret_cast<uintptr_t>(p.B) | static_cast<uintptr_t>(p.ldb)) & 15) == 0 ? p.K & ~15 : 0;
     const int8_t* rows[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) rows[r] = p.B + min(n0 + r, static_cast<long long>(p.N) - 1) * p.ldb;
     pdl_wait();
     pdl_launch_dependents();
-    uint4 w[R];
+    uint4 w[kDeep][R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) w[r] = load16(rows[r], 16 * lane, p.K, w_vec);
+    for (int d = 0; d < kDeep; ++d)
+#pragma unroll
+        for (int r = 0; r < R; ++r) w[d][r] = load16(rows[r], 16 * lane + 512 * d, kw_vec);
+
+    // lane r MT + m writes the value of channel r and token m
+    const int my_m = lane % MT;
+    const long long my_n = n0 + lane / MT;
+    const bool owns = lane < R * MT && my_m < p.M && my_n < p.N;
+    const float my_scale = owns ? p.b_scale[my_n] : 0.0f, my_bias = owns && p.bias ? p.bias[my_n] : 0.0f;
 
     // kPer threads on each token
     {
@@ -79,31 +85,41 @@ __global__ void __launch_bounds__(kFewThreads) i8_few_kernel(const TX* __restric
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[r][m] = 0;
-    for (int k = 16 * lane; k < p.K; k += 512) {
-        uint4 next[R];
+    for (int k0 = 16 * lane; k0 < kw_vec; k0 += 512 * kDeep) {
 #pragma unroll
-        for (int r = 0; r < R; ++r) next[r] = k + 512 < p.K ? load16(rows[r], k + 512, p.K, w_vec) : make_uint4(0, 0, 0, 0);
+        for (int d = 0; d < kDeep; ++d) {
+            const int k = k0 + 512 * d;
+            if (k < kw_vec) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const uint4 a = *reinterpret_cast<const uint4*>(xq + m * k16 + k);
+                for (int m = 0; m < MT; ++m) {
+                    const uint4 a = *reinterpret_cast<const uint4*>(xq + m * k16 + k);
 #pragma unroll
-            for (int r = 0; r < R; ++r) acc[r][m] = dot16(a, w[r], acc[r][m]);
+                    for (int r = 0; r < R; ++r) acc[r][m] = dot16(a, w[d][r], acc[r][m]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) w[d][r] = load16(rows[r], k + 512 * kDeep, kw_vec);
         }
-#pragma unroll
-        for (int r = 0; r < R; ++r) w[r] = next[r];
     }
+    for (int k = kw_vec + lane; k < p.K; k += 32) {        // the last K % 16 values; all of them for unaligned weights
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[r][m] += rows[r][k] * xq[m * k16 + k];
+    }
+    int mine = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
             const int sum = __reduce_add_sync(0xffffffffu, acc[r][m]);
-            const long long n = n0 + r;
-            if (lane == r * MT + m && n < p.N && m < p.M) {
-                float y = i8_epilogue(sum, scales[m], p.b_scale[n], p.bias ? p.bias[n] : 0.0f, p.act);
-                if (p.gate) y *= to_f32(static_cast<const TC*>(p.gate)[m * p.ld_gate + n]);
-                static_cast<TC*>(p.C)[m * p.ldc + n] = from_f32<TC>(y);
-            }
+            mine = lane == r * MT + m ? sum : mine;
         }
+    if (owns) {
+        float y = i8_epilogue(mine, scales[my_m], my_scale, my_bias, p.act);
+        if (p.gate) y *= to_f32(static_cast<const TC*>(p.gate)[my_m * p.ld_gate + my_n]);
+        static_cast<TC*>(p.C)[my_m * p.ldc + my_n] = from_f32<TC>(y);
+    }
 }
 
 template <typename TX, typename TC, int MT, int R>
@@ -114,13 +130,11 @@ cudaError_t launch_r(const TX* x, long long ld_x, const I8Product& p, cudaStream
 }
 template <typename TX, typename TC, int MT>
 cudaError_t launch_m(const TX* x, long long ld_x, const I8Product& p, cudaStream_t st) {
-    // About two blocks an SM: every block quantizes the tokens again, and every warp should have its weights on the way at once.
-    // Measured with 1 and with 4 channels a warp: 1 x 1024 -> 1024 2.5 and 3.2 us, 3 x 2048 -> 2048 4.6 and 6.7, 1 x 4096 -> 8192
-    // 14.6 and 10.4.
-    const long long blocks = 2ll * num_sms();
-    if (p.N <= kFewWarps * blocks) return launch_r<TX, TC, MT, 1>(x, ld_x, p, st);
-    if (p.N <= 2 * kFewWarps * blocks) return launch_r<TX, TC, MT, 2>(x, ld_x, p, st);
-    return launch_r<TX, TC, MT, 4>(x, ld_x, p, st);
+    // Two channels a warp: half the blocks quantize the tokens again, with 2 x 1 KB on the way for each warp; one channel a warp (four
+    // steps of it on the way) where the rows are long and the blocks are two an SM at most.  One and two channels measured: 1 x 1024 ->
+    // 1024 2.5 and 2.2 us, 1 x 1024 -> 8192 5.3 and 3.5, 4 x 2048 -> 8192 10.4 and 8.0; 1 x 4096 -> 2048 4.6 and 5.7, 4 x 2048 -> 1024
+    // 3.6 and 3.9.  Four channels gained 0.2 us at 4 x 1024 -> 4096 and lost as much elsewhere.
+    return p.K > 1024 && p.N <= 2 * kFewWarps * num_sms() ? launch_r<TX, TC, MT, 1>(x, ld_x, p, st) : launch_r<TX, TC, MT, 2>(x, ld_x, p, st);
 }
 template <typename TX, typename TC>
 int launch_x(const TX* x, long long ld_x, const I8Product& p, cudaStream_t st) {
@@ -136,8 +150,9 @@ int launch_c(const TX* x, long long ld_x, const I8Product& p, cudaStream_t st) {
 
 }  // namespace
 
-// Up to four tokens, as long as quantizing them in every block costs less than a kernel before the product: 2 x 4096 -> 8192 takes
-// 11.5 us this way and 11.2 in two kernels, 1 x 4096 -> 8192 10.4 and 11.1, 4 x 8192 -> 1024 15 and 8.
+// Up to four tokens, as long as quantizing them in every block costs less than a kernel before the product (us this way and in two
+// kernels): 4 x 2048 -> 1024 3.6 and 5.7, 4 x 2048 -> 8192 8.0 and 8.3, 2 x 4096 -> 8192 9.6 and 11.0; with 16384 values 4 x 4096 -> 4096
+// 9.6 and 8.4, 1 x 16384 -> 1024 11.9 and 10.4.
 bool i8_few(long long M, int K) { return M <= kI8Few && (M <= 2 ? M : 4) * ((K + 15ll) / 16 * 16) <= kI8FewValues; }
 
 int launch_i8_few(const void* x, int x_type, long long ld_x, const I8Product& p, cudaStream_t st) {
