@@ -286,8 +286,8 @@ int ppml_b200_flash_attn_forward_tokens(const ppml_b200_flash_cfg* cfg, int Lk, 
  * position beyond the table is never looked up: the token's rotated results (and gradients) are NaN.
  * Views: element (b, l, h, i) at p[b * sb + l * sl + h * sh + i]; Q, K and results may be strided in any way (ranges of a fused
  * projection, [B][L][h][d], [B][h][L][d]), inputs also with stride 0; elements of a result must lie apart (status 1), and a
- * result may be its own input's memory with the same strides.  hq and hk may
- * differ; one of them may be 0 (its views NULL).  d up to 512 (beyond: status 9), B * L below 2^31.
+ * result may be its own input's memory with the same strides and otherwise shares no element with any other operand or result.
+ * hq and hk may differ; one of them may be 0 (its views NULL).  d up to 512 (beyond: status 9), B * L below 2^31.
  * The backward pass takes the forward's inputs and the results' gradients dQo, dKo and writes dQ, dK (both sides, all of it) and,
  * where the pointers are given, dq_weight / dk_weight [d] fp32 (they are overwritten, and summed in a fixed order).  Those need a
  * workspace of ppml_b200_qk_norm_rope_backward_workspace(cfg) bytes, 16-byte aligned, used on `stream` only while the call

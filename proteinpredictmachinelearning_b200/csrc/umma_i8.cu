@@ -136,6 +136,19 @@ template <typename T, int MORE> struct Gates {
     }
 };
 
+// Columns of TMEM in eights, enough for `left` (1 to 32) tokens; the rest of r stays undefined.  Each way waits for itself: until
+// then nothing may touch the registers, a move where the ways meet included.
+__device__ __forceinline__ void load_sums8(uint32_t at, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_sums(uint32_t at, int left, uint32_t (&r)[32]) {
+    if (left > 24) { tmem_ld32(at, r); tmem_ld_wait(); }
+    else if (left > 16) { load_sums8(at, r); load_sums8(at + 8, r + 8); load_sums8(at + 16, r + 16); tmem_ld_wait(); }
+    else if (left > 8) { load_sums8(at, r); load_sums8(at + 8, r + 8); tmem_ld_wait(); }
+    else { load_sums8(at, r); tmem_ld_wait(); }
+}
+
 // The sums of `left` tokens (>= 32: all) from t0 on in this lane's channel n become results and go to C, eight tokens at a time.
 // MORE: 0 nothing follows, 1 an activation, 2 a gate (and perhaps an activation): instances of their own, because the registers of the
 // gates and the code of the five activations cost the plain ones a fifth of their time.  16-bit results in rows on 4 bytes go
@@ -167,49 +180,47 @@ __device__ __forceinline__ void finish_chunk(const I8Product& p, const uint32_t 
     const bool odd = lane & 1;
     uint32_t* to = reinterpret_cast<uint32_t*>(c + (odd ? ldc - 1 : 0));       // two channels of one token
     const uint32_t pick = odd ? 0x3276 : 0x5410;
-    auto store_paired = [&](int j0, const float (&y)[8]) {
+    const int mine = left - (odd ? 1 : 0);         // a lane's own token of two is there
+    auto store_paired = [&](int j0, const float (&y)[8], bool all) {
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const uint32_t own = narrow2(y[j], y[j + 1], T()), other = __shfl_xor_sync(0xffffffffu, own, 1);
-                to[ldc / 2 * (j0 + j)] = __byte_perm(own, other, pick);
+                if (all || j0 + j < mine) to[ldc / 2 * (j0 + j)] = __byte_perm(own, other, pick);
             }
         }
     };
-    const bool paired = sizeof(T) == 2 && left >= 32 && n - lane + 32 <= p.N && ((reinterpret_cast<uintptr_t>(p.C) >> 1 | p.ldc) & 1) == 0;
-    if (MORE > 0) {                                // one copy of the activations
+    auto store = [&](int j0, const float (&y)[8], bool all) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (all || j0 + j < left) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
+    };
+    const bool paired = sizeof(T) == 2 && n - lane + 32 <= p.N && ((reinterpret_cast<uintptr_t>(p.C) >> 1 | p.ldc) & 1) == 0;
+    // One copy of the activations for whole chunks, whose stores have no masks (65536 x 256 -> 256 sigmoid 22.2 -> 19.5 us), one for others.
+    if (MORE > 0 && left >= 32) {
 #pragma unroll
         for (int j0 = 0; j0 < 32; j0 += 8) {
             float y[8];
             results(j0, y);
-            if (paired) {
-                store_paired(j0, y);
-            } else if (n < p.N) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j0 + j < left) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
-            }
+            if (paired) store_paired(j0, y, true);
+            else if (n < p.N) store(j0, y, true);
         }
-    } else if (paired) {
+    } else if (left >= 32) {
+        if (paired) {
 #pragma unroll
-        for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y); store_paired(j0, y); }
-    } else if (n < p.N) {
-        if (left >= 32) {
+            for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y); store_paired(j0, y, true); }
+        } else if (n < p.N) {
 #pragma unroll
-            for (int j0 = 0; j0 < 32; j0 += 8) {
+            for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y); store(j0, y, true); }
+        }
+    } else {
+#pragma unroll
+        for (int j0 = 0; j0 < 32; j0 += 8) {
+            if (j0 < left) {
                 float y[8];
                 results(j0, y);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
-            }
-        } else {
-#pragma unroll
-            for (int j0 = 0; j0 < 32; j0 += 8) {
-                float y[8];
-                results(j0, y);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j0 + j < left) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
+                if (paired) store_paired(j0, y, false);
+                else if (n < p.N) store(j0, y, false);
             }
         }
     }
@@ -332,34 +343,35 @@ i8_tiles_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             const long long t0 = static_cast<long long>(tt) * q.bn;
             const long long rest = q.p.M - t0;
             const int cols = static_cast<int>(rest < q.bn ? rest : q.bn);
+            // This warp's tokens of the tile: a fourth, in chunks of 32 at most.  Where an activation follows the fourth is counted in
+            // eights (48 x 1024 -> 4096 GELU: 6.0 us in whole chunks, 5.0), else in whole chunks, which need no masks (65536 x 256 ->
+            // 256 bf16 12.8 us, 13.7 in eights).
+            constexpr int kGrain = MORE > 0 ? 8 : 32;
+            const int share = (cols + kGrain * kEpiParts - 1) / (kGrain * kEpiParts) * kGrain, first = part * share, mine = min(share, cols - first);
             float scale[2];                        // of the chunks this warp will read, requested before the wait
             Gates<T, MORE> gate;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int c = (part + k * kEpiParts) * 32 + lane;
-                scale[k] = c < cols ? q.p.a_scale[t0 + c] : 0.0f;
-            }
-            gate.load(q.p, t0 + part * 32, cols - part * 32, n);
+            for (int k = 0; k < 2; ++k) scale[k] = lane + 32 * k < mine ? q.p.a_scale[t0 + first + 32 * k + lane] : 0.0f;
+            gate.load(q.p, t0 + first, min(mine, 32), n);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull(acc), aph, cta_abort, q.err, 0x840 | acc))) break;
             tc_fence_after();
-            const uint32_t d = tmem + acc * (q.tmem_cols / 2) + (static_cast<uint32_t>(quarter * 32) << 16);
+            const uint32_t d = tmem + acc * (q.tmem_cols / 2) + (static_cast<uint32_t>(quarter * 32) << 16) + first;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int c = (part + k * kEpiParts) * 32;
+                const int left = min(32, mine - 32 * k);
                 uint32_t r[32];
-                if (c < cols) {
-                    if (k == 1) gate.load(q.p, t0 + c, cols - c, n);
+                if (left > 0) {
+                    if (k == 1) gate.load(q.p, t0 + first + 32, left, n);
                     __syncwarp();
-                    tmem_ld32(d + c, r);
-                    tmem_ld_wait();
+                    load_sums(d + 32 * k, left, r);
                 }
                 // the last read of this warp, or none in this tile: the accumulator may be written again
-                if (k == (part * 32 + 32 * kEpiParts < cols ? 1 : 0)) {
+                if (k == (mine > 32 ? 1 : 0)) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) { if (CG == 2) mbar_arrive_cluster(map_to(tempty(acc), 0)); else mbar_arrive(tempty(acc)); }
                 }
-                if (c < cols) finish_chunk<T, MORE>(q.p, r, gate, scale_buf, scale[k], t0 + c, cols - c, n, bs, bias, lane);
+                if (left > 0) finish_chunk<T, MORE>(q.p, r, gate, scale_buf, scale[k], t0 + first + 32 * k, left, n, bs, bias, lane);
             }
             if (++acc == 2) { acc = 0; aph ^= 1u; }
         }
@@ -451,16 +463,20 @@ i8_parts_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     if (warp >= kFirstEpi) {
         if (__all_sync(0xffffffffu, mbar_wait(tfull, 0, cta_abort, q.err, 0x940))) {
             tc_fence_after();
-            const int c = part * 32;               // bn <= 128: at most one chunk per warp
-            if (c < cols) {
+            // a fourth of the tile's tokens in eights: 32 at most, since bn <= 128
+            const int share = (cols + 8 * kEpiParts - 1) / (8 * kEpiParts) * 8, c = part * share, left = min(share, cols - c);
+            if (left > 0) {
                 uint32_t r[32];
                 __syncwarp();
-                tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, r);
-                tmem_ld_wait();
+                load_sums(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + c, left, r);
                 // the stages are free: every load has landed and every MMA has read
                 uint32_t* buf = reinterpret_cast<uint32_t*>(gen) + c * kRowsA + quarter * 32 + lane;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) buf[j * kRowsA] = r[j];
+                for (int j0 = 0; j0 < 32; j0 += 8)
+                    if (j0 < left) {
+#pragma unroll
+                        for (int j = j0; j < j0 + 8; ++j) buf[j * kRowsA] = r[j];
+                    }
             }
         }
     }
