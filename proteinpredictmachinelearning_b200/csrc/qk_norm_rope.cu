@@ -223,11 +223,11 @@ __global__ void __launch_bounds__(32 * kWarps) qk_backward_kernel(const QkParams
 // them, of different tokens: each group of lanes walks over the heads of its token, so that the position, its table row and
 // all but one addition of an address are had once per token instead of once per row.  A block works on one side (Q or K).
 // What bounds it: the bytes in flight.  Rows wait in registers from the load to the store, and 16 (bf16) to 24 (fp32) warps an SM are
-// what that leaves; a ring of rows in shared memory (cp.async) kept more in flight and cost 40 instructions a row: 120 against
-// 122 us on the long case below, 43 against 34 on the short one, and was dropped.
-// Measured (forward): 65536 tokens x 16 heads of 32, fp32 45 us (5.9 TB/s); 32768 tokens x 40 heads of 128, bf16 124 us (5.4 TB/s);
-// 16384 tokens x 32 heads of 64, bf16, LayerNorm, neighbouring pairs 35 us; backward of the last 54 us (3.8 TB/s), of 16384 tokens x 16
-// heads of 32, fp32 25 us.
+// what that leaves; a ring of rows in shared memory (cp.async) kept more in flight and cost 40 instructions a row: at an earlier
+// step 120 against 122 us on the long case below, 43 against 34 on the short one, and was dropped.
+// Measured (forward): 65536 tokens x 16 heads of 32, fp32 44 us (6.1 TB/s); 32768 tokens x 40 heads of 128, bf16 115 us (5.9 TB/s);
+// 16384 tokens x 32 heads of 64, bf16, LayerNorm, neighbouring pairs 30 us; backward of the last 47 us (4.3 TB/s), of 16384 tokens x 16
+// heads of 32, fp32 23 us.
 constexpr int kHeadsAtOnce = 4;                    // rows of a group of lanes that are loaded together (forward)
 
 template <int VB> struct RawOf;
@@ -676,8 +676,8 @@ cudaError_t launch_vec(const QkParams& p, QkVec& v, bool backward, cudaStream_t 
     const long long tokens = static_cast<long long>(p.B) * p.L;
     // An item is a token with all heads of a side, or, where tokens are few, with some of them.  What an item costs beside its rows
     // (position, table, factors: about two rows' work) speaks for long ones, even shares of the resident warps for many.
-    // Measured on 16384 tokens x 16 heads of 64 (bf16): forward 34.8 us from 24 items' warps an SM, 36.1 from 96; backward,
-    // whose grid is what is resident, 58.8 and 53.7.
+    // Measured on 16384 tokens x 16 heads of 64 (bf16): forward 30.0 us from 24 items' warps an SM, 31.1 from 48; backward,
+    // whose grid is what is resident, 51.5 from 24 and 47.1 from 96.
     const long long wanted = (backward ? 96ll : 24ll) * sms * W;
     long long warps[2];
     for (int k = 0; k < 2; ++k) {
