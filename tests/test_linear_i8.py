@@ -246,6 +246,35 @@ def test_linear_is_quantizer_and_product(M, dtype, no_device_abort):
 
 
 @gpu
+@pytest.mark.parametrize("M", [5, 7, 8, 15, 23, 25, 32, 40, 41, 56, 63, 72, 95, 97, 104, 120, 127, 136, 161, 192, 200, 223, 225, 239, 256, 257, 450])
+@pytest.mark.parametrize("act,K", [("silu", 64), ("relu", 64), ("none", 64), ("sigmoid", 1024)])
+def test_every_share_of_a_tile(M, act, K, no_device_abort):
+    """Tiles whose tokens fall unevenly to the warps of the epilogue, rows on and off the width of a paired store."""
+    A, W = ints(M, K, 1), ints(256, K, 2)
+    sa, sw = scales(M, 3) * (0.1 / K ** 0.5), scales(256, 4) * 10
+    for N, dtype, pitch in ((256, BF16, 256), (130, F16, 133), (256, F32, 257)):
+        gate = rows(M, N, dtype, 5)
+        out = torch.full((M + 1, pitch), -7.0, device="cuda", dtype=dtype)
+        for g in (None, gate):
+            ops.mul_mat_i8(A, sa, W[:N], sw[:N], gate=g, act=act, out=out[:M, :N])
+            check_product(out[:M, :N], A, sa, W[:N], sw[:N], None, g, act)
+        assert (out[M] == -7).all() and (out[:, N:] == -7).all()
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+@pytest.mark.parametrize("K", [1, 15, 17, 496, 511, 513, 1024, 1025, 1536, 2047, 2048])
+def test_few_tokens_at_the_ends_of_a_step(M, K, no_device_abort):
+    for N, pitch, shift in ((1, None, 0), (15, None, 0), (2367, None, 0), (2385, None, 0), (4741, None, 0), (100, K + 1, 3)):
+        x, W, ws, bias = rows(M, K, BF16, M, K + 3, 1), ints(N, K, 2, pitch, shift), scales(N, 3), scales(N, 4)
+        q, s = ops.quantize_tokens_i8(x)
+        out = torch.full((M + 1, N + 1), -7.0, device="cuda")
+        ops.linear_i8(x, W, ws, bias=bias, out=out[:M, :N])
+        assert torch.equal(out[:M, :N], ops.mul_mat_i8(q, s, W, ws, bias=bias, path=PATH_SIMT))
+        assert (out[M] == -7).all() and (out[:, N] == -7).all()
+
+
+@gpu
 @pytest.mark.parametrize("M,K,N", [(2, 272, 200), (30, 2048, 136), (300, 272, 264), (9000, 80, 300)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_gate_may_be_the_output(M, K, N, dtype, no_device_abort):
