@@ -121,8 +121,8 @@ __device__ __forceinline__ float i8_act(int kind, float x) {
         default: return x;
     }
 }
-// N values with one branch on the kind.  (Four values by a call that is not inlined took 80 cycles a value more, a branch per
-// value filled the instruction cache.)
+// N values with one branch on the kind, or with none where it is a constant.  (Four values by a call that is not inlined took 80 cycles
+// a value more, a branch per value filled the instruction cache.)
 template <int N> __device__ __forceinline__ void i8_act_all(int kind, float (&y)[N]) {
 #define PPML_ACT(K) case K: { _Pragma("unroll") for (int j = 0; j < N; ++j) y[j] = i8_act(K, y[j]); break; }
     switch (kind) { PPML_ACT(1) PPML_ACT(2) PPML_ACT(3) PPML_ACT(4) PPML_ACT(5) default: break; }

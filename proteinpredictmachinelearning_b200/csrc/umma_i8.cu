@@ -10,7 +10,7 @@
 //
 // What bounds it: with a long K the tensor pipe (16384 x 4096 -> 8192 335 us, 3.28 PFLOP/s, twice what cuBLAS reaches in bf16; back to
 // back the power limit takes it to some 400), with a short one the results' way out: 65536 x 256 -> 512 fp32 27 us (5.6 TB/s),
-// -> 1024 bf16 36 us (4.2 TB/s: issue of the epilogue, a third of it conversions), with SiLU 62 us (two transcendental instructions
+// -> 1024 bf16 36 us (4.2 TB/s: issue of the epilogue, a third of it conversions), with SiLU 52 us (two transcendental instructions
 // an output are 30 us alone); with few tokens the weights' way in: 48 x 4096 -> 8192 10.4 us cold (3.3 TB/s over 128 CTAs).
 #include <atomic>
 
@@ -149,9 +149,12 @@ __device__ __forceinline__ void load_sums(uint32_t at, int left, uint32_t (&r)[3
     else { load_sums8(at, r); tmem_ld_wait(); }
 }
 
+// an activation's number as a type
+template <int V> struct Kind { static constexpr int value = V; };
+
 // The sums of `left` tokens (>= 32: all) from t0 on in this lane's channel n become results and go to C, eight tokens at a time.
 // MORE: 0 nothing follows, 1 an activation, 2 a gate (and perhaps an activation): instances of their own, because the registers of the
-// gates and the code of the five activations cost the plain ones a fifth of their time.  16-bit results in rows on 4 bytes go
+// gates and the code of the activations cost the plain ones a fifth of their time.  16-bit results in rows on 4 bytes go
 // out two channels a lane: neighbouring lanes exchange one of two tokens, an even lane keeps its first token and takes the
 // neighbour's, an odd one the second.
 template <typename T, int MORE>
@@ -163,7 +166,7 @@ __device__ __forceinline__ void finish_chunk(const I8Product& p, const uint32_t 
     const uint64_t b2 = pack2(b_scale, b_scale), bias2 = pack2(bias, bias);
     T* c = static_cast<T*>(p.C) + t0 * p.ldc + n;
     const uint64_t ldc = static_cast<uint32_t>(p.ldc);         // below 2^32 (the launcher's condition): one multiply-add per address
-    auto results = [&](int j0, float (&y)[8]) {
+    auto results = [&](int j0, float (&y)[8], auto kind) {
 #pragma unroll
         for (int j = 0; j < 8; j += 4) {
             const float4 s = reinterpret_cast<const float4*>(scale_buf)[(j0 + j) / 4];
@@ -171,7 +174,7 @@ __device__ __forceinline__ void finish_chunk(const I8Product& p, const uint32_t 
             unpack2(ffma2(fmul2(pack2(f(0), f(1)), pack2(s.x, s.y)), b2, bias2), y[j], y[j + 1]);
             unpack2(ffma2(fmul2(pack2(f(2), f(3)), pack2(s.z, s.w)), b2, bias2), y[j + 2], y[j + 3]);
         }
-        if constexpr (MORE > 0) i8_act_all(p.act, y);
+        if constexpr (MORE > 0) i8_act_all(kind.value, y);
         if constexpr (MORE == 2) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] *= gate.at(j0 + j);
@@ -180,13 +183,12 @@ __device__ __forceinline__ void finish_chunk(const I8Product& p, const uint32_t 
     const bool odd = lane & 1;
     uint32_t* to = reinterpret_cast<uint32_t*>(c + (odd ? ldc - 1 : 0));       // two channels of one token
     const uint32_t pick = odd ? 0x3276 : 0x5410;
-    const int mine = left - (odd ? 1 : 0);         // a lane's own token of two is there
-    auto store_paired = [&](int j0, const float (&y)[8], bool all) {
+    auto store_paired = [&](int j0, const float (&y)[8]) {
         if constexpr (sizeof(T) == 2) {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const uint32_t own = narrow2(y[j], y[j + 1], T()), other = __shfl_xor_sync(0xffffffffu, own, 1);
-                if (all || j0 + j < mine) to[ldc / 2 * (j0 + j)] = __byte_perm(own, other, pick);
+                to[ldc / 2 * (j0 + j)] = __byte_perm(own, other, pick);
             }
         }
     };
@@ -196,32 +198,33 @@ __device__ __forceinline__ void finish_chunk(const I8Product& p, const uint32_t 
             if (all || j0 + j < left) c[ldc * (j0 + j)] = from_f32<T>(y[j]);
     };
     const bool paired = sizeof(T) == 2 && n - lane + 32 <= p.N && ((reinterpret_cast<uintptr_t>(p.C) >> 1 | p.ldc) & 1) == 0;
-    // One copy of the activations for whole chunks with one kind of store and no masks, one for the others (65536 x 256 -> 256 fp32
-    // sigmoid 22.2 -> 19.6 us; 65536 x 256 -> 1024 bf16 GELU 85 us with both kinds of stores behind a branch, 72).
-    if (MORE > 0 && left >= 32 && (sizeof(T) == 2 ? paired : n - lane + 32 <= p.N)) {
+    // Each loop has one kind of store, and no masks on a whole chunk: 65536 x 256 -> 256 fp32 sigmoid 22.2 -> 19.6 us; 65536 x 256 -> 1024
+    // bf16 GELU 85 us with both kinds of stores behind a branch, 72; 1999 x 1000 -> 777 fp16 SiLU and gate 8.5 and 8.1.
+    auto run = [&](auto kind) {
+        if (left >= 32 && paired) {
 #pragma unroll
-        for (int j0 = 0; j0 < 32; j0 += 8) {
-            float y[8];
-            results(j0, y);
-            if constexpr (sizeof(T) == 2) store_paired(j0, y, true); else store(j0, y, true);
-        }
-    } else if (MORE == 0 && left >= 32) {
-        if (paired) {
-#pragma unroll
-            for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y); store_paired(j0, y, true); }
+            for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y, kind); store_paired(j0, y); }
         } else if (n < p.N) {
+            if ((MORE == 0 || sizeof(T) == 4) && left >= 32) {     // 16 bits with an activation: one copy of it less
 #pragma unroll
-            for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y); store(j0, y, true); }
-        }
-    } else {
+                for (int j0 = 0; j0 < 32; j0 += 8) { float y[8]; results(j0, y, kind); store(j0, y, true); }
+            } else {
 #pragma unroll
-        for (int j0 = 0; j0 < 32; j0 += 8) {
-            if (j0 < left) {
-                float y[8];
-                results(j0, y);
-                if (paired) store_paired(j0, y, false);
-                else if (n < p.N) store(j0, y, false);
+                for (int j0 = 0; j0 < 32; j0 += 8)
+                    if (j0 < left) { float y[8]; results(j0, y, kind); store(j0, y, false); }
             }
+        }
+    };
+    if constexpr (MORE == 0) {
+        run(Kind<0>());
+    } else {                                       // the kind known to the loops: 65536 x 256 -> 1024 bf16 SiLU 60 -> 52 us, GELU 71 -> 58
+        switch (p.act) {
+            case 0: run(Kind<0>()); break;
+            case 1: run(Kind<1>()); break;
+            case 2: run(Kind<2>()); break;
+            case 3: run(Kind<3>()); break;
+            case 4: run(Kind<4>()); break;
+            default: run(Kind<5>());
         }
     }
     __syncwarp();
