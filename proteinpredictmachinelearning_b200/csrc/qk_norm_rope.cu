@@ -272,13 +272,14 @@ template <typename T, int VB> __device__ __forceinline__ Lane lane_of(const QkVe
     n.at_a = static_cast<uint32_t>(a * VB); n.at_b = static_cast<uint32_t>(b * VB);
     return n;
 }
-// cos and sin of the lane's pairs; NaN beyond the table; 1 and 0 where nothing turns
+// cos and sin of the lane's pairs; NaN beyond the table; 1 and 0 where nothing turns and, without a look-up, at a negative position
+// (padding, and lanes without an item): a row that no token names may hold anything, and 0 times a NaN would reach the weight gradients
 template <int V> __device__ __forceinline__ void load_table(const QkVec& v, const Lane& n, int pos, float (&c)[V], float (&s)[V]) {
     const int half = v.rot / 2;
     const float none = pos >= v.table_rows ? __uint_as_float(0x7fffffffu) : 1.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) { c[i] = i < n.turning ? none : 1.0f; s[i] = 0.0f; }
-    if (n.turning == 0 || pos >= v.table_rows) return;
+    if (n.turning == 0 || pos < 0 || pos >= v.table_rows) return;
     const long long at = static_cast<long long>(pos) * half + n.pair;
     if (V % 4 == 0 && v.table_vec) {
 #pragma unroll
@@ -509,7 +510,7 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_forward_kernel(const __gri
         };
         load(0);                                               // before the table, whose row waits for the position
         uint64_t c[V], s[V];
-        factors<V>(v, n, max(m.pos, 0), weights, c, s);
+        factors<V>(v, n, m.pos, weights, c, s);
         for (int h = 0;;) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(256, BLOCKS) qk_vec_backward_kernel(const __gr
         };
         load(0);                                   // before the table, whose row waits for the position
         float c[V], s[V];
-        load_table<V>(v, n, max(m.pos, 0), c, s);
+        load_table<V>(v, n, m.pos, c, s);
         for (int h = 0;;) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
