@@ -166,8 +166,10 @@ int ppml_b200_repack_q8_0(const void* blocks34_dev, int64_t nblocks, void* q8_0r
  * The CUDA-core product takes N up to 4194240 (status 9).
  * linear_i8 quantizes X on the way; one to four tokens of a short K (up to 8192, 4096 for two tokens, 2048 for three and four) run in
  * one kernel on the CUDA cores (path UMMA: status 7) and need no workspace (ppml_b200_linear_i8_workspace gives 0).  C shares no
- * element with X; gate may be C.  workspace: device memory of ppml_b200_linear_i8_workspace(M, K) bytes, 16-byte aligned,
- * used on `stream` only while the call runs there.  M = 0 is a call without work (status 0). */
+ * element with X where that one kernel runs, since its blocks read X while others write C (status 1); elsewhere X is quantized
+ * before C is written.  gate may be C (the same elements); results share no element with any other operand.  workspace: device
+ * memory of ppml_b200_linear_i8_workspace(M, K) bytes, 16-byte aligned, used on `stream` only while the call runs there.
+ * M = 0 is a call without work (status 0). */
 #define PPML_B200_TYPE_F32 0
 #define PPML_B200_TYPE_F16 1
 #define PPML_B200_TYPE_BF16 2

@@ -302,6 +302,17 @@ int check_i8(const int8_t* B, int64_t ldb, const float* b_scale, const void* C, 
     if (M > 0 && (!C || !aligned(C, type_bytes(c_type)) || !aligned(gate, type_bytes(c_type)))) return ST_BAD_ARGS;
     return ST_OK;
 }
+// Whether two matrices of M rows each (row lengths wa, wb and pitches pa, pb in bytes; the rows of either lie apart) share a byte.
+bool rows_meet(const void* a, int64_t pa, int64_t wa, const void* b, int64_t pb, int64_t wb, int64_t M) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    for (int64_t i = 0, j = 0; i < M && j < M;) {
+        const uintptr_t ai = a0 + static_cast<uintptr_t>(i * pa), bj = b0 + static_cast<uintptr_t>(j * pb);
+        if (ai + static_cast<uintptr_t>(wa) <= bj) ++i;
+        else if (bj + static_cast<uintptr_t>(wb) <= ai) ++j;
+        else return true;
+    }
+    return false;
+}
 int i8_product(const I8Product& p, int path, cudaStream_t st) {
     if (path != PPML_B200_PATH_SIMT) {
         const int rc = launch_umma_i8(p, st);
@@ -345,6 +356,9 @@ int ppml_b200_linear_i8(const void* X, int x_type, int64_t ld_x, const int8_t* B
     if (!X || !aligned(X, type_bytes(x_type))) return ST_BAD_ARGS;
     if (i8_few(M, K)) {
         if (path == PPML_B200_PATH_UMMA) return ST_UNSUPPORTED_PATH;
+        // every block reads all of X while others already write C
+        const int64_t ex = type_bytes(x_type), ec = type_bytes(c_type);
+        if (rows_meet(X, ld_x * ex, K * ex, C, ldc * ec, N * ec, M)) return ST_BAD_ARGS;
         return launch_i8_few(X, x_type, ld_x, I8Product{nullptr, B, 0, ldb, nullptr, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act}, as_stream(stream));
     }
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < ppml_b200_linear_i8_workspace(M, K)) return ST_SCRATCH;

@@ -159,6 +159,13 @@ PyObject* mul_mat_i8(PyObject* const* a) {
     return give(p.out, a[9]);
 }
 
+// Whether the memory from the first to the last element of two matrices has a byte in common.
+bool ranges_meet(const at::Tensor& a, int64_t pitch_a, const at::Tensor& b, int64_t pitch_b) {
+    auto bytes = [](const at::Tensor& t, int64_t p) { return static_cast<uintptr_t>(((t.size(0) - 1) * p + t.size(1)) * t.element_size()); };
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.data_ptr()), b0 = reinterpret_cast<uintptr_t>(b.data_ptr());
+    return a0 < b0 + bytes(b, pitch_b) && b0 < a0 + bytes(a, pitch_a);
+}
+
 // linear_i8(x, W, w_scale, bias, gate, act, dtype, path, out) -> out
 PyObject* linear_i8(PyObject* const* a) {
     const at::Tensor& x = activations(a[0]);
@@ -170,6 +177,18 @@ PyObject* linear_i8(PyObject* const* a) {
     const int64_t need = ppml_b200_linear_i8_workspace(M, p.K);
     at::Tensor ws;
     if (need) ws = fresh({need}, {1}, at::kByte, dev);
+    // An `out` around x itself: the one kernel for a few tokens reads x until its end, so the integers are made first.
+    if (!need && M > 0 && a[8] != Py_None && p.path != PPML_B200_PATH_UMMA && ranges_meet(x, ld, p.out, p.ldc)) {
+        const int64_t row = (K + 15) / 16 * 16;
+        ws = fresh({M * row}, {1}, at::kChar, dev);
+        const at::Tensor scale = fresh({M}, {1}, at::kFloat, dev);
+        int8_t* q = static_cast<int8_t*>(ws.data_ptr());
+        float* s = static_cast<float*>(scale.data_ptr());
+        check(ppml_b200_quantize_tokens_i8(x.data_ptr(), type_code(x.scalar_type()), ld, q, row, s, M, p.K, stream_of(dev)), "linear_i8");
+        check(ppml_b200_mul_mat_i8(q, row, s, p.w_ptr(), p.ldb, p.w_scale, p.out.data_ptr(), p.ldc, p.c_type, p.M, p.K, p.N, p.bias, p.gate_ptr(), p.ld_gate,
+                                   p.act, p.path, stream_of(dev)), "linear_i8");
+        return give(p.out, a[8]);
+    }
     check(ppml_b200_linear_i8(x.data_ptr(), type_code(x.scalar_type()), ld, p.w_ptr(), p.ldb, p.w_scale, p.out.data_ptr(), p.ldc, p.c_type, p.M, p.K, p.N,
                               p.bias, p.gate_ptr(), p.ld_gate, p.act, p.path, need ? ws.data_ptr() : nullptr, need, stream_of(dev)), "linear_i8");
     return give(p.out, a[8]);

@@ -206,13 +206,13 @@ def quantize_tokens_i8(x, out=None):
 def mul_mat_i8(A, a_scale, W, w_scale, bias=None, gate=None, act="none", dtype=torch.float32, path=PATH_AUTO, out=None):
     """act(a_scale[m] * w_scale[n] * sum_k A[m, k] W[n, k] + bias[n]) * gate[m, n]: A int8 [M, K] and W int8 [N, K] with their
     scales (quantize_tokens_i8), exact int32 sums, fp32 behind them, one rounding to `dtype` (of out and gate).  Rows of every
-    matrix are contiguous, at any pitch."""
+    matrix are contiguous, at any pitch; `out` may be the gate itself and otherwise shares no memory with an operand."""
     return (_native or _host()).mul_mat_i8(A, a_scale, W, w_scale, bias, gate, act, dtype, path, out)
 
 
 def linear_i8(x, W, w_scale, bias=None, gate=None, act="none", dtype=None, path=PATH_AUTO, out=None):
     """quantize_tokens_i8 and mul_mat_i8 as one call: x [M, K] fp32, fp16 or bf16; the result has x's type unless `dtype` (or
-    `out`) says otherwise."""
+    `out`) says otherwise.  `out` may share memory with x, or be the gate itself."""
     return (_native or _host()).linear_i8(x, W, w_scale, bias, gate, act, dtype, path, out)
 
 
@@ -229,7 +229,8 @@ def qk_norm_rope(Q, K, q_weight=None, k_weight=None, norm="rms", eps=1e-6, cos=N
     a fused projection, transposed views of [B, h, L, d]; one of them may be None), times q_weight / k_weight [d], then the
     rotation of the first 2 * cos.shape[1] dims by row `positions` (int32 [B, L] or [L]; None: 0, 1, ...) of cos / sin
     (rope_table).  A token with a negative position is padding and left alone.  Returns (Q', K'): `out` (tensors of the inputs'
-    shapes and types, any strides; the inputs themselves for a pass in place; None for a new one), or new [B, L, h, d] tensors."""
+    shapes and types, any strides; the inputs themselves for a pass in place, and otherwise no memory of another operand or result;
+    None for a new one), or new [B, L, h, d] tensors."""
     q, k = out if out is not None else (None, None)
     return (_native or _host()).qk_norm_rope(Q, K, q_weight, k_weight, norm, eps, cos, sin, positions, interleaved, q, k)
 
