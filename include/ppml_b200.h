@@ -157,9 +157,12 @@ int ppml_b200_repack_q8_0(const void* blocks34_dev, int64_t nblocks, void* q8_0r
  *   C[m][n]  = act(a_scale[m] * b_scale[n] * sum_k A[m][k] * B[n][k] + bias[n]) * gate[m][n]
  * A row of zeros has scale 0; a row that holds an infinity or a NaN has scale NaN and integers 0, so that its results are
  * NaN and no other row's are touched.  The sum is exact for every K up to PPML_B200_I8_MAX_K (beyond: status 9), whatever
- * the kernel; integers of -128 are fine.  Results are computed in fp32 and rounded once to c_type.  act as in
- * ppml_b200_mul_mat_f32_fused (NaN stays NaN under each); bias (fp32) and gate (c_type) may be NULL.  Every matrix has a row pitch in elements (ld_*,
- * >= its row length; elements behind a row are neither read into results nor written).
+ * the kernel; integers of -128 are fine.  Results are computed in fp32, fma(sum * a_scale, b_scale, bias) first, and rounded
+ * once to c_type.  act as in ppml_b200_mul_mat_f32_fused (NaN stays NaN under each).  Under path SIMT sigmoid, SiLU and GELU are
+ * its formulas in fp32; under AUTO and UMMA they go through the hardware's exponential and reciprocal: at v, the argument of the
+ * sigmoid, off by up to (8 + 2 |v|) 2^-24 of the value (GELU (8 + 8 |v|) 2^-24), and 0 for v < -87.3.  bias (fp32) and gate (c_type)
+ * may be NULL.  Every matrix has a row pitch in elements (ld_*, >= its row length; elements behind a row are neither read into
+ * results nor written).
  * quantize_tokens_i8 serves weights too: a row of W is an output channel.
  * path: AUTO / UMMA use the tensor cores where A and B are 16-byte aligned with pitches that are multiples of 16 bytes
  * (UMMA: status 7 otherwise), SIMT the CUDA cores; the sums are the same, so the results agree bit for bit for act = 0.

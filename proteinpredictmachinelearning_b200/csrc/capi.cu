@@ -338,7 +338,7 @@ int ppml_b200_mul_mat_i8(const int8_t* A, int64_t lda, const float* a_scale, con
     if (lda < K || !aligned(bias, 4)) return ST_BAD_ARGS;
     if (M == 0) return ST_OK;
     if (!A || !a_scale || !aligned(a_scale, 4)) return ST_BAD_ARGS;
-    const I8Product p{A, B, lda, ldb, a_scale, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act};
+    const I8Product p{A, B, lda, ldb, a_scale, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act, path == PPML_B200_PATH_SIMT};
     return i8_product(p, path, as_stream(stream));
 }
 
@@ -359,7 +359,7 @@ int ppml_b200_linear_i8(const void* X, int x_type, int64_t ld_x, const int8_t* B
         // every block reads all of X while others already write C
         const int64_t ex = type_bytes(x_type), ec = type_bytes(c_type);
         if (rows_meet(X, ld_x * ex, K * ex, C, ldc * ec, N * ec, M)) return ST_BAD_ARGS;
-        return launch_i8_few(X, x_type, ld_x, I8Product{nullptr, B, 0, ldb, nullptr, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act}, as_stream(stream));
+        return launch_i8_few(X, x_type, ld_x, I8Product{nullptr, B, 0, ldb, nullptr, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act, path == PPML_B200_PATH_SIMT}, as_stream(stream));
     }
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < ppml_b200_linear_i8_workspace(M, K)) return ST_SCRATCH;
     int8_t* q = static_cast<int8_t*>(workspace);
@@ -367,7 +367,7 @@ int ppml_b200_linear_i8(const void* X, int x_type, int64_t ld_x, const int8_t* B
     float* scale = reinterpret_cast<float*>(q + M * ld);
     const int rc = launch_quantize_tokens(X, x_type, ld_x, q, ld, scale, M, K, as_stream(stream));
     if (rc != ST_OK) return rc;
-    const I8Product p{q, B, ld, ldb, scale, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act};
+    const I8Product p{q, B, ld, ldb, scale, b_scale, bias, C, gate, ldc, ld_gate, M, N, K, c_type, act, path == PPML_B200_PATH_SIMT};
     return i8_product(p, path, as_stream(stream));
 }
 

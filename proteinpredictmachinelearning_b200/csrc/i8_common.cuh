@@ -102,9 +102,11 @@ template <typename T> __device__ __forceinline__ void quantize_vec(const uint4& 
     i8_quantize_all(x, scale, inv, q);
 }
 
-// The activations of act_scalar with sigmoid, SiLU and GELU through the hardware's exp2 and reciprocal (about 2 ulp each, the
-// exponent's argument rounded once; expf and an IEEE division cost a dozen instructions more per output):
-// 0.5 x (1 + tanh(u)) = x * sigmoid(2 u).  tanh itself stays exact: 2 sigmoid(2 x) - 1 would cancel near 0.
+// The activations of act_scalar with sigmoid, SiLU and GELU through the hardware's exp2 and reciprocal (expf and an IEEE division
+// cost a dozen instructions more per output): 0.5 x (1 + tanh(u)) = x * sigmoid(2 u).  tanh itself stays exact: 2 sigmoid(2 x) - 1
+// would cancel near 0.  With u = 2^-24: exp2 is off by 4 u, the sum by u, the reciprocal by 2 u, the last product by u, and the
+// exponent's argument by 1.22 u of itself, so that sigmoid(v) and SiLU are off by at most (8 + 2 |v|) u of their value, and GELU, whose
+// v has five roundings and a constant more, by (8 + 8 |v|) u.  Below v = -87.3 the reciprocal is subnormal and flushed: 0.
 __device__ __forceinline__ float i8_sigmoid(float x) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * x));
@@ -121,6 +123,16 @@ __device__ __forceinline__ float i8_act(int kind, float x) {
         default: return x;
     }
 }
+// The same with CUDA's expf and IEEE divisions, which PATH_SIMT asks for: at most 8 u (GELU: (8 + 8 |v|) u) down to v = -88.7, where
+// expf overflows.
+__device__ __forceinline__ float i8_act_exact(int kind, float x) {
+    switch (kind) {
+        case 1: return 1.0f / (1.0f + expf(-x));
+        case 2: return x / (1.0f + expf(-x));
+        case 3: return x / (1.0f + expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+        default: return i8_act(kind, x);
+    }
+}
 // N values with one branch on the kind, or with none where it is a constant.  (Four values by a call that is not inlined took 80 cycles
 // a value more, a branch per value filled the instruction cache.)
 template <int N> __device__ __forceinline__ void i8_act_all(int kind, float (&y)[N]) {
@@ -128,8 +140,9 @@ template <int N> __device__ __forceinline__ void i8_act_all(int kind, float (&y)
     switch (kind) { PPML_ACT(1) PPML_ACT(2) PPML_ACT(3) PPML_ACT(4) PPML_ACT(5) default: break; }
 #undef PPML_ACT
 }
-__device__ __forceinline__ float i8_epilogue(int sum, float a_scale, float b_scale, float bias, int act) {
-    return i8_act(act, fmaf(static_cast<float>(sum) * a_scale, b_scale, bias));
+__device__ __forceinline__ float i8_epilogue(int sum, float a_scale, float b_scale, float bias, const I8Product& p) {
+    const float y = fmaf(static_cast<float>(sum) * a_scale, b_scale, bias);
+    return p.exact ? i8_act_exact(p.act, y) : i8_act(p.act, y);
 }
 
 }  // namespace ppml_b200

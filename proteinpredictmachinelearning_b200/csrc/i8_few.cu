@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kFewThreads) i8_few_kernel(const TX* __restric
             mine = lane == r * MT + m ? sum : mine;
         }
     if (owns) {
-        float y = i8_epilogue(mine, scales[my_m], my_scale, my_bias, p.act);
+        float y = i8_epilogue(mine, scales[my_m], my_scale, my_bias, p);
         if (p.gate) y *= to_f32(static_cast<const TC*>(p.gate)[my_m * p.ld_gate + my_n]);
         static_cast<TC*>(p.C)[my_m * p.ldc + my_n] = from_f32<TC>(y);
     }

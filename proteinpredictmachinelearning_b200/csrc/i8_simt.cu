@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256) i8_dp4a_kernel(I8Product p) {
         for (int j = 0; j < 4; ++j) {
             const long long n = n0 + tx + 16 * j;
             if (n >= p.N) continue;
-            float y = i8_epilogue(acc[i][j], sa, p.b_scale[n], p.bias ? p.bias[n] : 0.0f, p.act);
+            float y = i8_epilogue(acc[i][j], sa, p.b_scale[n], p.bias ? p.bias[n] : 0.0f, p);
             if (p.gate) y *= to_f32(static_cast<const T*>(p.gate)[m * p.ld_gate + n]);
             static_cast<T*>(p.C)[m * p.ldc + n] = from_f32<T>(y);
         }

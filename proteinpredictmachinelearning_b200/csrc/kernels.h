@@ -130,6 +130,7 @@ struct I8Product {
     void* C; const void* gate;         // [M][N] of c_type with pitches ldc, ld_gate; gate may be null
     long long ldc, ld_gate;
     int M, N, K, c_type, act;
+    int exact;                         // activations through expf and divisions (CUDA cores only)
 };
 int launch_quantize_tokens(const void* x, int type, long long ld_x, int8_t* q, long long ld_q, float* scale, long long rows, int K,
                            cudaStream_t st);

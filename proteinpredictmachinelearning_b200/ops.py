@@ -205,7 +205,8 @@ def quantize_tokens_i8(x, out=None):
 
 def mul_mat_i8(A, a_scale, W, w_scale, bias=None, gate=None, act="none", dtype=torch.float32, path=PATH_AUTO, out=None):
     """act(a_scale[m] * w_scale[n] * sum_k A[m, k] W[n, k] + bias[n]) * gate[m, n]: A int8 [M, K] and W int8 [N, K] with their
-    scales (quantize_tokens_i8), exact int32 sums, fp32 behind them, one rounding to `dtype` (of out and gate).  Rows of every
+    scales (quantize_tokens_i8), exact int32 sums, fp32 behind them, one rounding to `dtype` (of out and gate).  Sigmoid,
+    SiLU and GELU go through the hardware's exponential and reciprocal, or under PATH_SIMT through fp32 formulas.  Rows of every
     matrix are contiguous, at any pitch; `out` may be the gate itself and otherwise shares no memory with an operand."""
     return (_native or _host()).mul_mat_i8(A, a_scale, W, w_scale, bias, gate, act, dtype, path, out)
 

@@ -1,11 +1,11 @@
-"""Linears in 8-bit integers at the edges: results that share memory with the input."""
+"""Linears in 8-bit integers at the edges: results that share memory with the input, activations over their whole range."""
 import ctypes as C
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from proteinpredictmachinelearning_b200 import PATH_AUTO, PATH_SIMT  # noqa: E402
+from proteinpredictmachinelearning_b200 import PATH_AUTO, PATH_SIMT, PATH_UMMA  # noqa: E402
 from proteinpredictmachinelearning_b200 import ops  # noqa: E402
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -50,3 +50,51 @@ def test_result_may_share_memory_with_the_input(M, K, dtype):
         buf[:, :K] = x
         assert torch.equal(ops.linear_i8(buf[:, :K], W, ws, bias=bias, path=path, out=buf[:, K + 8:]), want)
         assert torch.equal(buf[:, :K], x) and not buf[:, K:K + 8].any()
+
+
+# ---- activations over their whole range --------------------------------------------------------------------------------
+U = 2.0 ** -24
+
+
+def act_of(v, act):
+    """The value, and the argument of its sigmoid, in 64 bits."""
+    v = v.double()
+    s = v if act != "gelu" else 2 * 0.7978845608028654 * (v + 0.044715 * v ** 3)
+    return (1 if act == "sigmoid" else v) / (1 + torch.exp(-s)), s
+
+
+def reach(act, lowest):
+    """Arguments on either side whose sigmoid takes arguments from `lowest` to 200."""
+    v = torch.cat((torch.linspace(lowest, 12, 20001, device="cuda"), torch.linspace(12, 200, 501, device="cuda"), 10.0 ** torch.linspace(-30, 0, 61, device="cuda"),
+                   -(10.0 ** torch.linspace(-30, 0, 61, device="cuda"))))
+    if act == "gelu":
+        v = v.clamp(-20, 20)
+    return v[act_of(v, act)[1] >= lowest]
+
+
+@gpu
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("path,lowest,slope", [(PATH_SIMT, -88.5, 0), (PATH_UMMA, -87.0, 2), (PATH_AUTO, -87.0, 2)])
+def test_activations_of_the_product(act, path, lowest, slope):
+    """One integer 1 on either side: the token's scale goes into the activation as it is.  expf is off by 2 units in the last place
+    (4 u), the sum and the division by u each; the hardware's functions as the header says; GELU's argument has seven
+    roundings of itself.  What is below the smallest normal number may be off by a step there."""
+    v = reach(act, lowest)
+    A, W = torch.ones((v.numel(), 16), device="cuda", dtype=torch.int8)[:, :1], torch.ones((3, 16), device="cuda", dtype=torch.int8)[:, :1]
+    want, s = act_of(v, act)
+    tol = (8 + (8 if act == "gelu" else slope) * s.abs()) * U * want.abs() + (2.0 ** -126 if slope else 2.0 ** -148)
+    y = ops.mul_mat_i8(A, v, W, torch.ones(3, device="cuda"), act=act, path=path)
+    assert ((y.double() - want[:, None]).abs() <= tol[:, None]).all(), ((y.double() - want[:, None]).abs() / tol[:, None]).max()
+
+
+@gpu
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("path,lowest,slope", [(PATH_SIMT, -88.5, 0), (PATH_AUTO, -87.0, 2)])
+def test_activations_of_a_few_tokens(act, path, lowest, slope):
+    """The one kernel for a few tokens: its bias goes into the activation as it is, behind a token of zeros."""
+    v = reach(act, lowest)
+    W, ws = torch.ones((v.numel(), 16), device="cuda", dtype=torch.int8), torch.ones(v.numel(), device="cuda")
+    want, s = act_of(v, act)
+    tol = (8 + (8 if act == "gelu" else slope) * s.abs()) * U * want.abs() + (2.0 ** -126 if slope else 2.0 ** -148)
+    y = ops.linear_i8(torch.zeros((3, 16), device="cuda"), W, ws, bias=v, act=act, path=path)
+    assert ((y.double() - want).abs() <= tol).all(), ((y.double() - want).abs() / tol).max()
