@@ -122,10 +122,11 @@ def load():
 
 
 def load_torch_binding():
-    """The CPython module over the library for torch tensors (csrc/torch_binding.cpp)."""
+    """The CPython module over the library for torch tensors (csrc/torch_binding.cpp), which uses torch's own functions and so belongs
+    to the torch it was built against."""
     import importlib.util
 
-    import torch  # noqa: F401  (its libraries have to be in the process)
+    import torch
     if not os.path.exists(TORCH_BINDING_PATH):
         raise ImportError(
             f"{TORCH_BINDING_PATH} is missing: build it with `python -m proteinpredictmachinelearning_b200.build` "
@@ -133,4 +134,7 @@ def load_torch_binding():
     spec = importlib.util.spec_from_file_location("ppml_b200_torch", TORCH_BINDING_PATH)
     module = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(module)
+    if module.torch_version != torch.__version__:
+        raise ImportError(f"{TORCH_BINDING_PATH} was built against torch {module.torch_version}, {torch.__version__} is installed: "
+                          "build it again with `python -m proteinpredictmachinelearning_b200.build`")
     return module

@@ -330,4 +330,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "ppml_b200_torch", nullptr, -1, met
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_ppml_b200_torch(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_ppml_b200_torch(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", PPML_TORCH_VERSION) != 0) { Py_DECREF(m); return nullptr; }
+    return m;
+}
