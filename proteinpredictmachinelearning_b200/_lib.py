@@ -8,8 +8,6 @@ LIB_PATH = os.path.join(_HERE, "lib", "libppml_b200.so")
 
 PATH_AUTO, PATH_SIMT, PATH_UMMA = 0, 1, 2
 TF32_ROUND, TF32_TMA, TF32_TRUNCATE = 0, 1, 2
-TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
-I8_MAX_K = 131071                    # PPML_B200_I8_MAX_K
 NOALLOC_SCRATCH_BYTES = 4 << 20      # PPML_B200_NOALLOC_SCRATCH_BYTES
 
 
