@@ -3,7 +3,8 @@
 // allocator on the current stream, one call into libppml_b200.so.  Done in Python, the same checks and the argument conversion of
 // ctypes take 7 to 14 us a call, several times what the kernels take for one token.
 //
-// Wrong tensors raise ValueError, a status of the library RuntimeError; no C++ exception leaves a function.
+// Wrong tensors raise ValueError, a status of the library RuntimeError, an allocation that fails torch.OutOfMemoryError; no C++ exception
+// leaves a function.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -307,6 +308,16 @@ PyObject* qk_norm_rope_backward(PyObject* const* a) {
     return four;
 }
 
+// torch's own class, which programs catch to go on with less; RuntimeError, its base, where it cannot be had
+void set_out_of_memory(const char* what) {
+    PyObject* torch = PyImport_ImportModule("torch");
+    PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+    if (!type) PyErr_Clear();
+    PyErr_SetString(type ? type : PyExc_RuntimeError, what);
+    Py_XDECREF(type);
+    Py_XDECREF(torch);
+}
+
 template <PyObject* (*F)(PyObject* const*), Py_ssize_t N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
     try {
@@ -314,6 +325,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return F(args);
     } catch (const Refused& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (const c10::OutOfMemoryError& e) {
+        set_out_of_memory(e.what_without_backtrace());
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_RuntimeError, e.what());
     } catch (...) {

@@ -1,4 +1,5 @@
-"""Linears in 8-bit integers at the edges: results that share memory with the input, activations over their whole range."""
+"""Linears in 8-bit integers at the edges: results that share memory with the input, activations over their whole range,
+results that no memory holds."""
 import ctypes as C
 
 import pytest
@@ -98,3 +99,13 @@ def test_activations_of_a_few_tokens(act, path, lowest, slope):
     tol = (8 + (8 if act == "gelu" else slope) * s.abs()) * U * want.abs() + (2.0 ** -126 if slope else 2.0 ** -148)
     y = ops.linear_i8(torch.zeros((3, 16), device="cuda"), W, ws, bias=v, act=act, path=path)
     assert ((y.double() - want).abs() <= tol).all(), ((y.double() - want).abs() / tol).max()
+
+
+# ---- memory ------------------------------------------------------------------------------------------------------------
+@gpu
+def test_a_result_that_no_memory_holds():
+    """4 TB: the allocator's own error, as from any torch call, and the next call runs."""
+    x, W, ws = rand((1 << 20, 16), 1), torch.ones((1 << 20, 16), device="cuda", dtype=torch.int8), torch.ones(1 << 20, device="cuda")
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.linear_i8(x, W, ws)
+    assert torch.equal(ops.linear_i8(x[:8], W[:8], ws[:8]), ops.linear_i8(x, W[:8], ws[:8])[:8])
