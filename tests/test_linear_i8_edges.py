@@ -1,5 +1,5 @@
 """Linears in 8-bit integers at the edges: results that share memory with the input, activations over their whole range,
-results that no memory holds."""
+results that no memory holds, and every cut of the product into tiles."""
 import ctypes as C
 
 import pytest
@@ -109,3 +109,77 @@ def test_a_result_that_no_memory_holds():
     with pytest.raises(torch.OutOfMemoryError):
         ops.linear_i8(x, W, ws)
     assert torch.equal(ops.linear_i8(x[:8], W[:8], ws[:8]), ops.linear_i8(x, W[:8], ws[:8])[:8])
+
+
+# ---- every cut of the product ------------------------------------------------------------------------------------------
+# Sizes at which the choice falls on each kind of tile, with ends of tiles of every length (tokens of a tile: sizes).
+PARTS = {  # clusters of two, four and eight CTAs that share a tile's K
+    "16": [(5, 1185, 4352), (5, 917, 40), (5, 2090, 40)],
+    "32": [(20, 2048, 8192), (1145, 1159, 43), (35, 994, 41), (18, 938, 40), (33, 1932, 41), (17, 2087, 40)],
+    "48": [(48, 4096, 8192), (35, 1697, 5142), (34, 1206, 2082), (33, 1928, 935)],
+    "64": [(200, 8192, 1024), (3459, 2462, 41), (3195, 2435, 46), (1287, 1823, 41), (1136, 1916, 41), (586, 3796, 45), (491, 3651, 42)],
+    "80": [(66, 3216, 5164), (69, 1862, 3250), (65, 2074, 1620)],
+    "96": [(4813, 2651, 52), (5246, 3079, 42), (2406, 2501, 49), (2955, 2239, 43), (1183, 2746, 43), (1141, 2563, 50)],
+    "112": [(100, 4987, 4769), (98, 2506, 2836), (105, 4885, 1047)],
+    "128": [(7819, 3988, 41), (7295, 4061, 52), (3207, 4032, 40), (3784, 3985, 40), (1537, 7849, 74), (1622, 7769, 41), (1649, 8249, 52)]}
+SINGLE = {  # one CTA a tile
+    "64": [(5005, 18, 40), (4833, 17, 46)], "96": [(10289, 16, 40), (9758, 17, 40), (9790, 16, 42)],
+    "128": [(14729, 16, 47), (15803, 16, 42), (15452, 16, 48), (14712, 16, 45)],
+    "160": [(22579, 21, 45), (22463, 19, 44), (20249, 17, 42), (20313, 16, 41)],
+    "192": [(8191, 64, 300), (27845, 16, 40), (24615, 18, 41), (24079, 18, 41), (26629, 16, 40), (23798, 16, 54)],
+    "224": [(10000, 64, 300), (30047, 20, 42), (30541, 17, 45), (28802, 18, 41), (30179, 16, 46), (28668, 20, 49)],
+    "256": [(5000, 64, 777), (34313, 16, 43), (34352, 18, 55), (36176, 23, 40), (35183, 16, 42), (36760, 16, 44), (33972, 17, 51), (33236, 17, 52),
+            (34807, 16, 75)]}
+PAIRS = {  # two CTAs a tile of 256 channels
+    "64": [(2589, 1412, 152), (2609, 1487, 136)], "96": [(4923, 948, 138), (4843, 986, 129), (5454, 961, 130)],
+    "128": [(7321, 738, 145), (7131, 757, 141), (7535, 682, 138)], "160": [(11364, 516, 129), (10809, 600, 131), (11196, 522, 154)],
+    "192": [(12700, 431, 165), (11991, 387, 130), (13428, 387, 135)], "224": [(15908, 505, 157), (15049, 408, 130), (15384, 443, 134), (16329, 419, 145)],
+    "256": [(17409, 258, 157), (16674, 265, 156), (16986, 308, 129), (16745, 257, 135), (18312, 266, 150), (16828, 289, 152), (450, 263, 6672),
+            (17893, 258, 167)]}
+
+
+def check(got, want, tol):
+    """NaN fails, in what is wanted too."""
+    assert torch.isfinite(want).all()
+    off = (got.double() - want).abs()
+    assert (off <= tol).all(), (int((~(off <= tol)).sum()), off.max().item())
+
+
+@pytest.fixture
+def no_device_abort():
+    yield
+    code, where = ops.device_status()
+    assert code == 0, f"a kernel gave up a bounded wait: code {code} at site {where:#x}"
+
+
+@gpu
+@pytest.mark.parametrize("kind,sizes", [(f"{k}-{t}", s) for k, d in (("parts", PARTS), ("single", SINGLE), ("pairs", PAIRS)) for t, s in d.items()],
+                         ids=lambda v: v if isinstance(v, str) else "")
+def test_every_cut(kind, sizes, no_device_abort):
+    """Each type with nothing, an activation, a gate, and both behind the sum, rows that lie close and rows that lie apart, against 64
+    bits.  The integer sum is exact; its conversion, two factors and the sum with the bias are 4 roundings of |product| + |bias|, which
+    an activation of slope 1.13 at most carries on; its own bound is (8 + 8 |v|) u of the result at worst, with |result| <= |v| and |v|
+    below 10 here; the gate and the stored type round once more each."""
+    for M, K, N in sizes:
+        g = torch.Generator(device="cuda").manual_seed(M + K + N)
+        draw = lambda *shape: torch.randn(shape, generator=g, device="cuda")     # noqa: E731
+        A, W = ((draw(n, (K + 15) // 16 * 16) * 40).round().clamp(-128, 127).to(torch.int8)[:, :K] for n in (M, N))
+        sa, sw, bias = draw(M).abs().clamp(0.1, 2) / (1600 * K ** 0.5), draw(N).abs().clamp(0.1, 2), draw(N)
+        prod = (A.double() @ W.double().t()) * sa.double()[:, None] * sw.double()
+        for dtype in (F32, F16, BF16):
+            half = torch.finfo(dtype).eps / 2
+            gate = draw(M, N + 2).to(dtype)[:, 1:N + 1]
+            for act, b, h, pitch in (("none", bias, None, N), ("none", None, gate, N + 3), ("silu", bias, None, (N + 1) // 2 * 2), ("silu", None, gate, N),
+                                     ("gelu", bias, gate, N + 5)):
+                x = prod if b is None else prod + b.double()
+                size = prod.abs() + (0 if b is None else b.double().abs())
+                v = x if act != "gelu" else 2 * 0.7978845608028654 * (x + 0.044715 * x ** 3)
+                want = x if act == "none" else x / (1 + torch.exp(-v))
+                tol = 1.13 * 4 * U * size + (0 if act == "none" else (8 + 8 * v.abs()) * U * want.abs())
+                if h is not None:
+                    want, tol = want * h.double(), tol * h.double().abs() + U * (want * h.double()).abs()
+                tol = tol * (1 + half) + half * want.abs() + torch.finfo(dtype).smallest_normal * half
+                out = torch.full((M + 1, pitch), -7.0, device="cuda", dtype=dtype)
+                ops.mul_mat_i8(A, sa, W, sw, bias=b, gate=h, act=act, out=out[:M, :N])
+                check(out[:M, :N], want, tol)
+                assert (out[M] == -7).all() and (out[:, N:] == -7).all()
