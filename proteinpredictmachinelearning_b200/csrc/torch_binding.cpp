@@ -99,10 +99,9 @@ PyObject* quantize_tokens_i8(PyObject* const* a) {
     const c10::Device dev = x.device();
     const c10::cuda::CUDAGuard guard(dev);
     const int64_t ld = pitch(x, x.scalar_type(), M, K, dev, "x");
-    const at::Tensor* given = optional_tensor(a[1], "q");
-    at::Tensor q, s;
-    if (given) { q = *given; s = tensor(a[2], "scale"); }
-    else { q = fresh({M, K}, {(K + 15) / 16 * 16, 1}, at::kChar, dev); s = fresh({M}, {1}, at::kFloat, dev); }
+    const at::Tensor* own_q = optional_tensor(a[1], "q");
+    const at::Tensor* own_s = optional_tensor(a[2], "scale");
+    const at::Tensor q = own_q ? *own_q : fresh({M, K}, {(K + 15) / 16 * 16, 1}, at::kChar, dev), s = own_s ? *own_s : fresh({M}, {1}, at::kFloat, dev);
     check(ppml_b200_quantize_tokens_i8(x.data_ptr(), type_code(x.scalar_type()), ld, static_cast<int8_t*>(q.data_ptr()), pitch(q, at::kChar, M, K, dev, "q"),
                                        const_cast<float*>(vec(&s, M, dev, "scale")), M, extent(K, "x"), stream_of(dev)), "quantize_tokens_i8");
     PyObject* two = PyTuple_New(2);

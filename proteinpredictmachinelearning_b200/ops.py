@@ -198,7 +198,8 @@ def _host():
 def quantize_tokens_i8(x, out=None):
     """x [M, K] (fp32, fp16 or bf16; rows contiguous, any pitch) -> (int8 [M, K], fp32 scales [M]): scale = max |x| / 127 of the
     row, q = round(x / scale).  New integers get a row pitch that is a multiple of 16 bytes, which the tensor-core product
-    wants.  Weights [N, K] are quantized the same way, one scale for each output channel.  `out`: a pair to write into."""
+    wants.  Weights [N, K] are quantized the same way, one scale for each output channel.  `out`: a pair to write into,
+    either of them None for a new one."""
     q, scale = out if out is not None else (None, None)
     return (_native or _host()).quantize_tokens_i8(x, q, scale)
 

@@ -111,6 +111,19 @@ def test_a_result_that_no_memory_holds():
     assert torch.equal(ops.linear_i8(x[:8], W[:8], ws[:8]), ops.linear_i8(x, W[:8], ws[:8])[:8])
 
 
+# ---- one of two results given ------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("M,K", [(3, 64), (40, 1000)])
+def test_quantizer_writes_into_what_it_is_given(M, K):
+    x = rand((M, K), 1, BF16)
+    q, s = ops.quantize_tokens_i8(x)
+    for give_q, give_s in ((True, True), (True, False), (False, True)):
+        mine = (torch.full((M, K), 77, device="cuda", dtype=torch.int8) if give_q else None, torch.full((M,), -7.0, device="cuda") if give_s else None)
+        got = ops.quantize_tokens_i8(x, out=mine)
+        assert torch.equal(got[0], q) and torch.equal(got[1], s)
+        assert all(m is None or m is t for m, t in zip(mine, got))
+
+
 # ---- every cut of the product ------------------------------------------------------------------------------------------
 # Sizes at which the choice falls on each kind of tile, with ends of tiles of every length (tokens of a tile: sizes).
 PARTS = {  # clusters of two, four and eight CTAs that share a tile's K
