@@ -111,9 +111,6 @@ __device__ __forceinline__ void issue_block(bool lead, uint32_t d, uint64_t desc
 }
 
 // ---- epilogue of 32 tokens x this lane's channel ----
-__device__ __forceinline__ uint32_t narrow2(float a, float b, __nv_bfloat16) { const __nv_bfloat162 t = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
-__device__ __forceinline__ uint32_t narrow2(float a, float b, __half) { const __half2 t = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&t); }
-
 // Gates of 32 tokens, requested before their sums are there.
 template <typename T, int MORE> struct Gates {
     uint32_t w[MORE < 2 ? 1 : sizeof(T) == 2 ? 16 : 32];
