@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(THREADS) quantize_by_block_kernel(const T* __r
     if (threadIdx.x == 0) scale[row] = s;
 }
 
-// Any length, any alignment: one block per row, value by value; the second pass over the row comes from L1 / L2.
+// Any length, any alignment: one block per row, value by value; the second pass over the row comes from L1 / L2.  Bound by its narrow
+// loads: 1.1 TB/s in bf16 and 1.8 in fp32 at K = 4001 (6.8 at 4000), 1.8 in fp32 at K = 12288.
 template <typename T>
 __global__ void __launch_bounds__(512) quantize_any_kernel(const T* __restrict__ x, long long ld_x, int8_t* __restrict__ q, long long ld_q,
                                                            float* __restrict__ scale, int K) {
